@@ -300,6 +300,7 @@ def _plain_append(state):
         amax = torch.zeros(touched.numel(), kv, device=x.device).index_reduce_(0, where, size, "amax")
         needed = _needed_scale(amax, kind)
         old = scales[plane][touched]
+        needed = torch.where((before[:, None] > 0) & (amax == 0), old, needed)  # zeros fit any scale
         new = torch.where(before[:, None] > 0, torch.maximum(old, needed), needed)
         held = _bytes(codes[plane])[touched].view(codes.dtype)
         again = _encode(held.float() * (old / new)[..., None, None], kind)
@@ -427,7 +428,8 @@ def _exact_append(case, state):
                 x = source[start + first - (n - q):start + last - (n - q)].double().transpose(0, 1)
                 scale, block, old = _exact_scale(x, kind), table[r][b], first - b * page
                 if old:
-                    scale = torch.maximum(scale, scales[plane, block])
+                    zero = x.abs().amax((1, 2)) == 0
+                    scale = torch.where(zero, scales[plane, block], torch.maximum(scale, scales[plane, block]))
                     was = codes[plane, block, :, :old] * (scales[plane, block] / scale)[:, None, None]
                     codes[plane, block, :, :old] = _exact_code(was, kind)
                 codes[plane, block, :, old:old + last - first] = _exact_code(x / scale[:, None, None], kind)
