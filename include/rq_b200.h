@@ -296,6 +296,105 @@ int32_t rq_peer_close(void* mapped);
 /* Synchronizes `stream` and returns the status recorded in `state`: RQ_OK or RQ_ERR_DEVICE_TIMEOUT. */
 int32_t rq_peer_barrier_status(const void* state, void* stream);
 
+/* ---- 8-bit block-scaled KV cache ------------------------------------------------------------------------------------
+ * A paged cache for KV owners that are not residual-coded (no counterpart in the reference, which keeps them in bf16):
+ * one byte per channel and one fp32 scale per (plane, block, KV head).  A cached value is code * scale.
+ *   codes    e4m3 or int8 [2][num_blocks][kv_heads][page_tokens][head_dim], plane 0 = K, plane 1 = V
+ *   scales   fp32 [2][num_blocks][kv_heads]; rq_block_append and rq_block_evict write powers of two, attention reads any
+ *            positive finite value
+ *   weights  fp32 [num_blocks][kv_heads][page_tokens]: accumulated attention weight of every cached token, or NULL
+ * Token t of request r lives in block block_table[r][t / page_tokens] at slot t % page_tokens, for every KV head.
+ * No two requests of one call may share a block that the call writes.  A block id outside 0..num_blocks-1 is never
+ * dereferenced: tokens in such a block are invisible to attention, not written by append, and lost by evict. */
+typedef enum RqBlockElement { RQ_BLOCK_E4M3 = 0, RQ_BLOCK_INT8 = 1 } RqBlockElement;
+typedef enum RqActivation { RQ_ACTIVATION_BF16 = 0, RQ_ACTIVATION_FP16 = 1 } RqActivation;
+
+typedef struct RqBlockCache {
+    void* codes;   /* 16-byte aligned */
+    float* scales;
+    float* weights; /* or NULL */
+    int64_t num_blocks;
+    int32_t kv_heads;
+    int32_t head_dim;    /* 64, 96 or 128 */
+    int32_t page_tokens; /* 16 or 32 */
+    int32_t element;     /* RqBlockElement */
+} RqBlockCache;
+
+/* The batch of a step: rows query_start_loc[r] .. query_start_loc[r + 1] - 1 of the row tensors are the LAST tokens of
+ * request r, at positions seq_lens[r] - (number of rows) .. seq_lens[r] - 1; query_start_loc starts at 0 and never
+ * decreases.  Rows from query_start_loc[num_requests] on are padding. */
+typedef struct RqBlockBatch {
+    const int32_t* query_start_loc; /* [num_requests + 1] */
+    const int32_t* seq_lens;        /* [num_requests], the step's own tokens included */
+    const int32_t* block_table;     /* [>= num_requests][block_table_stride] */
+    int32_t num_requests;
+    int32_t block_table_stride;
+    int32_t max_blocks_per_request; /* block_table.size(1) */
+} RqBlockBatch;
+
+/* Quantize the step's K/V rows into their blocks.  The scale of a block is the smallest power of two (from 2^-100 on)
+ * that brings the largest finite magnitude of its tokens into the type's range (448 or 127); 1 where all are zero.  A call
+ * whose tokens join earlier ones of their block never lowers its scale, and rounds the earlier ones again when it grows.
+ * Rounding is to nearest even; infinities saturate, NaN becomes 0.  Slots that hold none of the request's tokens keep
+ * their bytes.  With cache.weights the new tokens' accumulated weights start at 0.  One launch. */
+typedef struct RqBlockAppendArgs {
+    RqBlockCache cache;
+    RqBlockBatch batch;
+    const void* key;   /* [num_rows][kv_heads][head_dim], last two dims packed, row strides in ELEMENTS */
+    const void* value;
+    int64_t key_stride, value_stride;
+    int32_t num_rows;
+    int32_t activation; /* RqActivation of key and value */
+    void* stream;
+    int32_t flags;      /* RQ_FLAG_SERIAL_LAUNCH */
+} RqBlockAppendArgs;
+int32_t rq_block_append(const RqBlockAppendArgs* args);
+
+/* Softmax attention of the step's rows over the cache, the step's own tokens included (append comes first): the row at
+ * position p sees the tokens 0..p of its request.  Query heads are shared out evenly: head h reads KV head
+ * h / (heads / kv_heads).  A row that sees no token gets zeros and lse = -inf; padding rows are left untouched.
+ * With accumulate every visible token's softmax weight, summed over the request's rows and the query heads of its KV
+ * head, is added to cache.weights. */
+typedef struct RqBlockAttentionArgs {
+    RqBlockCache cache;
+    RqBlockBatch batch;
+    const void* query;  /* [num_rows][heads][head_dim], last two dims packed, 16-byte aligned, row strides in ELEMENTS */
+    void* output;       /* like query */
+    int64_t query_stride, output_stride; /* multiples of 8 */
+    int32_t num_rows;
+    int32_t heads;
+    int32_t activation; /* RqActivation of query and output */
+    int32_t accumulate;
+    float softmax_scale;
+    float* lse;         /* fp32 [num_rows][heads], natural logarithm, or NULL */
+    int32_t max_seq_len; /* upper bound of seq_lens for this call, 0 = the page table's width; tokens from it on are not
+                            seen.  Only the size of the workspace of an accumulating call depends on it */
+    void* workspace;    /* rq_block_attention_workspace_bytes() bytes, 256-byte aligned; no initialisation needed */
+    size_t workspace_bytes;
+    void* stream;
+    int32_t flags;      /* RQ_FLAG_SERIAL_LAUNCH */
+} RqBlockAttentionArgs;
+/* Scratch one rq_block_attention call needs; workspace and workspace_bytes of the arguments are not looked at.  0 when
+ * the arguments are not valid. */
+size_t rq_block_attention_workspace_bytes(const RqBlockAttentionArgs* args);
+int32_t rq_block_attention(const RqBlockAttentionArgs* args);
+
+/* Bring every request of more than `budget` tokens down to `budget`: for each KV head on its own keep the first `sinks`
+ * tokens, the last `recent` ones, and of the others those with the largest accumulated weight (ties: the lowest position;
+ * NaN counts as lowest).  The kept tokens move, in their order, to positions 0 .. budget - 1 of the request's blocks, their
+ * weights with them; every block they fill gets the scale that its kept tokens need (the rule of rq_block_append).  Slots from
+ * position `budget` on keep their bytes.  query_start_loc of the batch is not used.  One launch. */
+typedef struct RqBlockEvictArgs {
+    RqBlockCache cache; /* weights required */
+    RqBlockBatch batch;
+    int32_t budget, sinks, recent; /* sinks + recent <= budget, budget >= 1 */
+    int32_t* kept;      /* int32 [num_requests][kv_heads][budget]: the positions that the kept tokens had, then -1 */
+    int32_t* new_lens;  /* int32 [num_requests]: min(seq_len, budget); not the memory of seq_lens; or NULL */
+    void* stream;
+    int32_t flags;      /* RQ_FLAG_SERIAL_LAUNCH */
+} RqBlockEvictArgs;
+int32_t rq_block_evict(const RqBlockEvictArgs* args);
+
 const char* rq_last_error(void);
 const char* rq_version(void);
 

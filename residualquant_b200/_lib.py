@@ -44,6 +44,10 @@ EXPORTS = (
     "rq_peer_export",
     "rq_peer_open",
     "rq_peer_close",
+    "rq_block_append",
+    "rq_block_attention",
+    "rq_block_attention_workspace_bytes",
+    "rq_block_evict",
     "rq_last_error",
     "rq_version",
 )
@@ -143,6 +147,81 @@ class RqPeerBarrierArgs(ctypes.Structure):
     ]
 
 
+class RqBlockCache(ctypes.Structure):
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_tokens", ctypes.c_int32),
+        ("element", ctypes.c_int32),
+    ]
+
+
+class RqBlockBatch(ctypes.Structure):
+    _fields_ = [
+        ("query_start_loc", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("num_requests", ctypes.c_int32),
+        ("block_table_stride", ctypes.c_int32),
+        ("max_blocks_per_request", ctypes.c_int32),
+    ]
+
+
+class RqBlockAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", RqBlockCache),
+        ("batch", RqBlockBatch),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_stride", ctypes.c_int64),
+        ("value_stride", ctypes.c_int64),
+        ("num_rows", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("stream", ctypes.c_void_p),
+        ("flags", ctypes.c_int32),
+    ]
+
+
+class RqBlockAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", RqBlockCache),
+        ("batch", RqBlockBatch),
+        ("query", ctypes.c_void_p),
+        ("output", ctypes.c_void_p),
+        ("query_stride", ctypes.c_int64),
+        ("output_stride", ctypes.c_int64),
+        ("num_rows", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("accumulate", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("lse", ctypes.c_void_p),
+        ("max_seq_len", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
+        ("flags", ctypes.c_int32),
+    ]
+
+
+class RqBlockEvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", RqBlockCache),
+        ("batch", RqBlockBatch),
+        ("budget", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+        ("kept", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p),
+        ("flags", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -197,6 +276,14 @@ def load() -> ctypes.CDLL:
     lib.rq_peer_open.restype = ctypes.c_int32
     lib.rq_peer_close.argtypes = [ctypes.c_void_p]
     lib.rq_peer_close.restype = ctypes.c_int32
+    lib.rq_block_append.argtypes = [ctypes.POINTER(RqBlockAppendArgs)]
+    lib.rq_block_append.restype = ctypes.c_int32
+    lib.rq_block_attention.argtypes = [ctypes.POINTER(RqBlockAttentionArgs)]
+    lib.rq_block_attention.restype = ctypes.c_int32
+    lib.rq_block_attention_workspace_bytes.argtypes = [ctypes.POINTER(RqBlockAttentionArgs)]
+    lib.rq_block_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.rq_block_evict.argtypes = [ctypes.POINTER(RqBlockEvictArgs)]
+    lib.rq_block_evict.restype = ctypes.c_int32
     lib.rq_last_error.argtypes = []
     lib.rq_last_error.restype = ctypes.c_char_p
     lib.rq_version.argtypes = []

@@ -33,9 +33,12 @@ UNITS = {
     "rq_attention_d128.cu": [],
     "rq_attention_d96.cu": [],
     "rq_peer.cu": [],
+    "rq_block_append.cu": [],
+    "rq_block_attention.cu": [],
+    "rq_block_evict.cu": [],
     "rq_capi.cu": [],
 }
-HEADERS = ["rq_common.cuh", "rq_kernels.h", "rq_attention_impl.cuh", os.path.join("..", "..", "include", "rq_b200.h")]
+HEADERS = ["rq_common.cuh", "rq_kernels.h", "rq_attention_impl.cuh", "rq_block_common.cuh", os.path.join("..", "..", "include", "rq_b200.h")]
 
 
 def nvcc() -> str:

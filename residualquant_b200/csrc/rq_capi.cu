@@ -629,4 +629,157 @@ int32_t rq_peer_barrier_status(const void* state, void* stream) {
     return RQ_OK;
 }
 
+// ---- 8-bit block-scaled cache ---------------------------------------------------------------------------------
+static int block_view(const RqBlockCache& c, const RqBlockBatch& b, bool rows, rq::BlockView* v) {
+    if (c.head_dim != 64 && c.head_dim != 96 && c.head_dim != 128)
+        return fail(RQ_ERR_UNSUPPORTED, "no block-cache kernel for head_dim=%d (64, 96 or 128)", c.head_dim);
+    if (c.page_tokens != 16 && c.page_tokens != 32)
+        return fail(RQ_ERR_UNSUPPORTED, "no block-cache kernel for page_tokens=%d (16 or 32)", c.page_tokens);
+    if (c.element != RQ_BLOCK_E4M3 && c.element != RQ_BLOCK_INT8)
+        return fail(RQ_ERR_UNSUPPORTED, "unknown block-cache element %d", c.element);
+    if (c.kv_heads < 1 || c.num_blocks < 1) return fail(RQ_ERR_INVALID_ARGUMENT, "a block cache needs at least one head and one block");
+    if (c.kv_heads > 65535 || c.num_blocks > 0x7fffffff) return fail(RQ_ERR_INVALID_ARGUMENT, "too many heads or blocks in one cache");
+    if (c.codes == nullptr || !aligned(c.codes, 16) || c.scales == nullptr || !aligned(c.scales, 4) || !aligned(c.weights, 4))
+        return fail(RQ_ERR_INVALID_ARGUMENT, "16-byte aligned 8-bit codes [2, blocks, heads, page tokens, channels] and fp32 scales required");
+    if (b.num_requests < 1 || b.seq_lens == nullptr || (b.block_table == nullptr && b.max_blocks_per_request > 0) || (rows && b.query_start_loc == nullptr))
+        return fail(RQ_ERR_INVALID_ARGUMENT, "int32 query starts [requests+1], sequence lengths [requests] and page table required");
+    if (b.max_blocks_per_request < 0 || b.block_table_stride < b.max_blocks_per_request || b.max_blocks_per_request > 0x7fffffff / 32)
+        return fail(RQ_ERR_INVALID_ARGUMENT, "int32 page table with packed rows required");
+    v->codes = static_cast<uint8_t*>(c.codes);
+    v->scales = c.scales;
+    v->weights = c.weights;
+    v->num_blocks = c.num_blocks;
+    v->kv_heads = c.kv_heads;
+    v->page_tokens = c.page_tokens;
+    v->query_start_loc = b.query_start_loc;
+    v->seq_lens = b.seq_lens;
+    v->block_table = b.block_table;
+    v->num_requests = b.num_requests;
+    v->table_stride = b.block_table_stride;
+    v->max_blocks = b.max_blocks_per_request;
+    return RQ_OK;
+}
+
+static int chained(int32_t flags) { return programmatic_launch_enabled() && !(flags & RQ_FLAG_SERIAL_LAUNCH) ? 1 : 0; }
+
+int32_t rq_block_append(const RqBlockAppendArgs* a) {
+    if (a == nullptr) return fail(RQ_ERR_INVALID_ARGUMENT, "null arguments");
+    rq::BlockAppendParams p;
+    memset(&p, 0, sizeof(p));
+    const int status = block_view(a->cache, a->batch, true, &p.v);
+    if (status != RQ_OK) return status;
+    if (a->num_rows < 0 || a->num_rows > 0x7fffffff / 64) return fail(RQ_ERR_INVALID_ARGUMENT, "row count %d out of range", a->num_rows);
+    if (a->num_rows == 0) return RQ_OK;
+    if (a->activation != RQ_ACTIVATION_BF16 && a->activation != RQ_ACTIVATION_FP16)
+        return fail(RQ_ERR_UNSUPPORTED, "unknown activation type %d", a->activation);
+    const int64_t row = static_cast<int64_t>(a->cache.kv_heads) * a->cache.head_dim;
+    if (a->key == nullptr || a->value == nullptr || !aligned(a->key, 2) || !aligned(a->value, 2) || a->key_stride < row ||
+        a->value_stride < row)
+        return fail(RQ_ERR_INVALID_ARGUMENT, "16-bit [tokens, heads, channels] with packed trailing strides required");
+    p.rows[0] = a->key;
+    p.rows[1] = a->value;
+    p.stride[0] = a->key_stride;
+    p.stride[1] = a->value_stride;
+    p.num_rows = a->num_rows;
+    p.fp16 = a->activation == RQ_ACTIVATION_FP16;
+    p.vector_loads = aligned(a->key, 16) && aligned(a->value, 16) && a->key_stride % 8 == 0 && a->value_stride % 8 == 0;
+    // Rows a warp walks over in search of the blocks that begin there: one while that leaves enough warps to fill the GPU
+    // (single-token steps), up to a block's worth for prompts, where only every page_tokens-th row begins a block.
+    p.chunk = 1;
+    while (p.chunk < a->cache.page_tokens &&
+           static_cast<int64_t>(a->num_rows) * 2 * a->cache.kv_heads / (2 * p.chunk) >= 16LL * current_sm_count())
+        p.chunk *= 2;
+    if ((static_cast<int64_t>(a->num_rows) + p.chunk - 1) / p.chunk * 2 * a->cache.kv_heads / 8 >= 0x7fffffffLL)
+        return fail(RQ_ERR_INVALID_ARGUMENT, "too many rows in one call");
+    p.programmatic_launch = chained(a->flags);
+    const cudaError_t err = rq::launch_block_append(p, a->cache.head_dim, a->cache.element == RQ_BLOCK_INT8, static_cast<cudaStream_t>(a->stream));
+    return err == cudaSuccess ? RQ_OK : fail_cuda(err, "block append launch");
+}
+
+static int block_attention_params(const RqBlockAttentionArgs* a, rq::BlockAttentionParams* p, size_t* workspace) {
+    memset(p, 0, sizeof(*p));
+    *workspace = 0;
+    const int status = block_view(a->cache, a->batch, true, &p->v);
+    if (status != RQ_OK) return status;
+    if (a->num_rows < 0) return fail(RQ_ERR_INVALID_ARGUMENT, "negative row count");
+    if (a->heads < 1 || a->heads % a->cache.kv_heads != 0)
+        return fail(RQ_ERR_INVALID_ARGUMENT, "%d query heads are no multiple of the cache's %d heads", a->heads, a->cache.kv_heads);
+    if (a->activation != RQ_ACTIVATION_BF16 && a->activation != RQ_ACTIVATION_FP16)
+        return fail(RQ_ERR_UNSUPPORTED, "unknown activation type %d", a->activation);
+    const int64_t row = static_cast<int64_t>(a->heads) * a->cache.head_dim;
+    if (a->num_rows > 0 &&
+        (a->query == nullptr || a->output == nullptr || !aligned(a->query, 16) || !aligned(a->output, 16) || a->query_stride < row ||
+         a->output_stride < row || a->query_stride % 8 != 0 || a->output_stride % 8 != 0))
+        return fail(RQ_ERR_INVALID_ARGUMENT, "16-byte aligned 16-bit [tokens, heads, channels] with packed trailing strides required");
+    if (!(a->softmax_scale > 0.f && a->softmax_scale < 1e30f)) return fail(RQ_ERR_INVALID_ARGUMENT, "softmax scale must be positive and finite");
+    if (a->max_seq_len < 0) return fail(RQ_ERR_INVALID_ARGUMENT, "negative max_seq_len");
+    if (a->accumulate && a->cache.weights == nullptr) return fail(RQ_ERR_INVALID_ARGUMENT, "accumulating needs a cache with weights");
+    if (static_cast<int64_t>(a->num_rows) * a->heads > 0x7fffffffLL / 64) return fail(RQ_ERR_INVALID_ARGUMENT, "too many query rows in one call");
+    p->query = a->query;
+    p->output = a->output;
+    p->query_stride = a->query_stride;
+    p->output_stride = a->output_stride;
+    p->num_rows = a->num_rows;
+    p->heads = a->heads;
+    p->group = a->heads / a->cache.kv_heads;
+    p->fp16 = a->activation == RQ_ACTIVATION_FP16;
+    p->accumulate = a->accumulate ? 1 : 0;
+    const int table_len = a->batch.max_blocks_per_request * a->cache.page_tokens;
+    p->max_len = a->max_seq_len != 0 && a->max_seq_len < table_len ? a->max_seq_len : table_len;
+    p->scale_log2 = a->softmax_scale * 1.4426950408889634f;
+    p->lse = a->lse;
+    *workspace = round_up(static_cast<size_t>(a->num_rows) * a->heads * sizeof(float), 256);
+    return RQ_OK;
+}
+
+size_t rq_block_attention_workspace_bytes(const RqBlockAttentionArgs* a) {
+    rq::BlockAttentionParams p;
+    size_t need = 0;
+    if (a == nullptr || block_attention_params(a, &p, &need) != RQ_OK) return 0;
+    return need;
+}
+
+int32_t rq_block_attention(const RqBlockAttentionArgs* a) {
+    if (a == nullptr) return fail(RQ_ERR_INVALID_ARGUMENT, "null arguments");
+    rq::BlockAttentionParams p;
+    size_t need = 0;
+    const int status = block_attention_params(a, &p, &need);
+    if (status != RQ_OK) return status;
+    if (a->num_rows == 0) return RQ_OK;
+    if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < need)
+        return fail(RQ_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu", need, a->workspace_bytes);
+    p.row_lse = static_cast<float*>(a->workspace);
+    p.programmatic_launch = chained(a->flags);
+    const cudaError_t err = rq::launch_block_attention(p, a->cache.head_dim, a->cache.element == RQ_BLOCK_INT8, static_cast<cudaStream_t>(a->stream));
+    return err == cudaSuccess ? RQ_OK : fail_cuda(err, "block attention launch");
+}
+
+int32_t rq_block_evict(const RqBlockEvictArgs* a) {
+    if (a == nullptr) return fail(RQ_ERR_INVALID_ARGUMENT, "null arguments");
+    rq::BlockEvictParams p;
+    memset(&p, 0, sizeof(p));
+    const int status = block_view(a->cache, a->batch, false, &p.v);
+    if (status != RQ_OK) return status;
+    if (a->cache.weights == nullptr) return fail(RQ_ERR_INVALID_ARGUMENT, "evicting needs a cache with weights");
+    if (a->budget < 1 || a->budget > 0x7fffffff / 64 || a->sinks < 0 || a->recent < 0 ||
+        static_cast<int64_t>(a->sinks) + a->recent > a->budget)
+        return fail(RQ_ERR_INVALID_ARGUMENT, "a budget of %d tokens cannot hold the first %d and the last %d", a->budget, a->sinks, a->recent);
+    if (a->kept == nullptr || !aligned(a->kept, 4) || !aligned(a->new_lens, 4))
+        return fail(RQ_ERR_INVALID_ARGUMENT, "int32 [requests, heads, budget] for the kept positions required");
+    if (a->new_lens == a->batch.seq_lens) return fail(RQ_ERR_INVALID_ARGUMENT, "new_lens must not be seq_lens itself");
+    const int64_t pairs = static_cast<int64_t>(a->batch.num_requests) * a->cache.kv_heads;
+    if (pairs > 0x7fffffffLL / 64) return fail(RQ_ERR_INVALID_ARGUMENT, "too many requests in one call");
+    p.budget = a->budget;
+    p.sinks = a->sinks;
+    p.recent = a->recent;
+    p.kept = a->kept;
+    p.new_lens = a->new_lens;
+    // CTAs per (request, KV head): up to eight while that keeps the grid within one wave of two CTAs per multiprocessor
+    p.cluster = 1;
+    while (p.cluster < 8 && pairs * p.cluster * 2 <= 2LL * current_sm_count()) p.cluster *= 2;
+    p.programmatic_launch = chained(a->flags);
+    const cudaError_t err = rq::launch_block_evict(p, a->cache.head_dim, a->cache.element == RQ_BLOCK_INT8, static_cast<cudaStream_t>(a->stream));
+    return err == cudaSuccess ? RQ_OK : fail_cuda(err, "block evict launch");
+}
+
 }  // extern "C"

@@ -121,4 +121,53 @@ struct AttentionVariant {
 cudaError_t launch_attention(const AttentionVariant& v, const AttentionParams& p, cudaStream_t stream);
 bool attention_variant_available(const AttentionVariant& v);
 
+// ---- 8-bit block-scaled cache (rq_block_*.cu) ----------------------------------------------------------------
+struct BlockView {
+    uint8_t* codes;
+    float* scales;
+    float* weights;          // or nullptr
+    int64_t num_blocks;
+    int kv_heads, page_tokens;
+    const int32_t* query_start_loc;
+    const int32_t* seq_lens;
+    const int32_t* block_table;
+    int num_requests, table_stride, max_blocks;
+};
+
+struct BlockAppendParams {
+    BlockView v;
+    const void* rows[2];     // key, value
+    int64_t stride[2];       // elements
+    int num_rows;
+    int fp16;                // activations are fp16 (else bf16)
+    int vector_loads;        // rows are 16-byte aligned
+    int chunk;               // rows that one warp walks over
+    int programmatic_launch;
+};
+cudaError_t launch_block_append(const BlockAppendParams& p, int head_dim, int int8, cudaStream_t stream);
+
+struct BlockAttentionParams {
+    BlockView v;
+    const void* query;
+    void* output;
+    int64_t query_stride, output_stride;
+    int num_rows, heads, group, fp16, accumulate;
+    int max_len;             // tokens from here on are not seen
+    float scale_log2;        // softmax scale * log2(e)
+    float* lse;              // or nullptr
+    float* row_lse;          // workspace [num_rows][heads]: log2 of the softmax denominator (accumulate)
+    int programmatic_launch;
+};
+cudaError_t launch_block_attention(const BlockAttentionParams& p, int head_dim, int int8, cudaStream_t stream);
+
+struct BlockEvictParams {
+    BlockView v;
+    int budget, sinks, recent;
+    int32_t* kept;
+    int32_t* new_lens;       // or nullptr
+    int cluster;             // CTAs per (request, KV head)
+    int programmatic_launch;
+};
+cudaError_t launch_block_evict(const BlockEvictParams& p, int head_dim, int int8, cudaStream_t stream);
+
 }  // namespace rq

@@ -1,0 +1,106 @@
+"""Refusals and sizes of the block cache's C ABI, and the cache class without a GPU (CPU)."""
+
+import ctypes
+
+import pytest
+import torch
+
+from residualquant_b200 import _lib
+from residualquant_b200.block_cache import BlockCache
+
+ADDRESS = 1 << 20   # a pointer that is only looked at
+
+
+def append_args(**changes):
+    cache = dict(codes=ADDRESS, scales=ADDRESS, weights=ADDRESS, num_blocks=8, kv_heads=2, head_dim=128, page_tokens=16, element=0)
+    batch = dict(query_start_loc=ADDRESS, seq_lens=ADDRESS, block_table=ADDRESS, num_requests=2, block_table_stride=4, max_blocks_per_request=4)
+    rest = dict(key=ADDRESS, value=ADDRESS, key_stride=256, value_stride=256, num_rows=0, activation=0)
+    return _fill(_lib.RqBlockAppendArgs, cache, batch, rest, changes)
+
+
+def attention_args(**changes):
+    cache = dict(codes=ADDRESS, scales=ADDRESS, weights=ADDRESS, num_blocks=8, kv_heads=2, head_dim=128, page_tokens=16, element=0)
+    batch = dict(query_start_loc=ADDRESS, seq_lens=ADDRESS, block_table=ADDRESS, num_requests=2, block_table_stride=4, max_blocks_per_request=4)
+    rest = dict(query=ADDRESS, output=ADDRESS, query_stride=1024, output_stride=1024, num_rows=3, heads=8, activation=0, accumulate=0,
+                softmax_scale=0.1)
+    return _fill(_lib.RqBlockAttentionArgs, cache, batch, rest, changes)
+
+
+def evict_args(**changes):
+    cache = dict(codes=ADDRESS, scales=ADDRESS, weights=ADDRESS, num_blocks=8, kv_heads=2, head_dim=128, page_tokens=16, element=0)
+    batch = dict(query_start_loc=None, seq_lens=ADDRESS, block_table=ADDRESS, num_requests=2, block_table_stride=4, max_blocks_per_request=4)
+    return _fill(_lib.RqBlockEvictArgs, cache, batch, dict(budget=0, sinks=0, recent=0, kept=ADDRESS, new_lens=None), changes)
+
+
+def _fill(kind, cache, batch, rest, changes):
+    for part in (cache, batch, rest):
+        part.update({k: v for k, v in changes.items() if k in part})
+    return kind(cache=_lib.RqBlockCache(**cache), batch=_lib.RqBlockBatch(**batch), **rest)
+
+
+BAD_CACHE = [dict(head_dim=80), dict(page_tokens=24), dict(element=2), dict(kv_heads=0), dict(num_blocks=0), dict(codes=None),
+             dict(codes=ADDRESS + 8), dict(scales=None), dict(num_requests=0), dict(seq_lens=None), dict(block_table=None),
+             dict(block_table_stride=3), dict(max_blocks_per_request=-1), dict(num_blocks=1 << 40)]
+
+
+@pytest.mark.parametrize("changes", BAD_CACHE + [dict(query_start_loc=None), dict(num_rows=-1)])
+def test_append_refuses(built_library, changes):
+    lib = _lib.load()
+    assert lib.rq_block_append(ctypes.byref(append_args())) == 0           # nothing to do, nothing launched
+    assert lib.rq_block_append(ctypes.byref(append_args(**changes))) < 0
+    assert lib.rq_last_error()
+
+
+@pytest.mark.parametrize("changes", [dict(key=None), dict(value=ADDRESS + 1), dict(key_stride=255), dict(activation=7),
+                                     dict(num_rows=0x7FFFFFFF)])
+def test_append_refuses_rows(built_library, changes):
+    lib = _lib.load()
+    assert lib.rq_block_append(ctypes.byref(append_args(**{"num_rows": 1, **changes}))) < 0
+    assert lib.rq_block_append(None) == -1
+
+
+@pytest.mark.parametrize("changes", BAD_CACHE + [
+    dict(query_start_loc=None), dict(heads=3), dict(heads=0), dict(query=None), dict(output=ADDRESS + 8), dict(query_stride=1023),
+    dict(output_stride=1028), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")), dict(softmax_scale=float("inf")),
+    dict(activation=2), dict(num_rows=-1), dict(num_rows=1 << 28), dict(accumulate=1, weights=None)])
+def test_attention_refuses(built_library, changes):
+    lib = _lib.load()
+    args = attention_args(**changes)
+    assert lib.rq_block_attention(ctypes.byref(args)) < 0
+    assert lib.rq_block_attention_workspace_bytes(ctypes.byref(args)) == 0
+    assert lib.rq_block_attention(None) == -1 and lib.rq_block_attention_workspace_bytes(None) == 0
+
+
+def test_attention_asks_for_its_workspace(built_library):
+    lib = _lib.load()
+    args = attention_args()
+    need = lib.rq_block_attention_workspace_bytes(ctypes.byref(args))
+    assert need > 0 and need % 256 == 0
+    assert lib.rq_block_attention(ctypes.byref(args)) == -3                 # none given
+    args.workspace, args.workspace_bytes = ADDRESS, need - 1
+    assert lib.rq_block_attention(ctypes.byref(args)) == -3
+    args.workspace, args.workspace_bytes = ADDRESS + 16, need
+    assert lib.rq_block_attention(ctypes.byref(args)) == -3
+    assert lib.rq_block_attention(ctypes.byref(attention_args(num_rows=0))) == 0
+    # the scores of an accumulating call: rows x heads x the length bound
+    counted = lib.rq_block_attention_workspace_bytes(ctypes.byref(attention_args(accumulate=1)))
+    assert counted >= need
+
+
+@pytest.mark.parametrize("changes", BAD_CACHE + [dict(weights=None), dict(), dict(budget=4, sinks=3, recent=2), dict(budget=4, sinks=-1),
+                                                 dict(budget=4, recent=-1), dict(budget=4, kept=None), dict(budget=4, kept=ADDRESS + 2),
+                                                 dict(budget=4, new_lens=ADDRESS), dict(budget=1 << 30)])
+def test_evict_refuses(built_library, changes):
+    lib = _lib.load()
+    if changes in BAD_CACHE:
+        changes = dict(budget=4, **changes)
+    assert lib.rq_block_evict(ctypes.byref(evict_args(**changes))) < 0
+    assert lib.rq_block_evict(None) == -1
+
+
+def test_the_cache_lives_on_the_gpu(built_library):
+    codes = torch.zeros(2, 4, 2, 16, 64, dtype=torch.int8)
+    with pytest.raises(RuntimeError):
+        BlockCache(codes, torch.ones(2, 4, 2))
+    with pytest.raises(RuntimeError):
+        BlockCache.allocate(4, 2, 64, device="cpu")
