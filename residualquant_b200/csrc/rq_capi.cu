@@ -728,7 +728,27 @@ static int block_attention_params(const RqBlockAttentionArgs* a, rq::BlockAttent
     p->max_len = a->max_seq_len != 0 && a->max_seq_len < table_len ? a->max_seq_len : table_len;
     p->scale_log2 = a->softmax_scale * 1.4426950408889634f;
     p->lse = a->lse;
-    *workspace = round_up(static_cast<size_t>(a->num_rows) * a->heads * sizeof(float), 256);
+    // Eight queries share a CTA's reads of the cache, sixteen where the requests have more (rows are taken to be spread
+    // evenly over the requests; any spread is right).
+    const int64_t rows_each = (static_cast<int64_t>(a->num_rows) + a->batch.num_requests - 1) / a->batch.num_requests;
+    p->query_tiles = rows_each * p->group <= 8 ? 1 : 2;
+    // One span for each resident CTA, fewer where the batch cannot have that many chunks.
+    const int64_t per_item = (static_cast<int64_t>(p->max_len) + rq::block_attention_chunk() - 1) / rq::block_attention_chunk();
+    const int64_t items = (static_cast<int64_t>(a->num_rows) * p->group / (8 * p->query_tiles) + a->batch.num_requests) * a->cache.kv_heads;
+    const int64_t resident = (p->query_tiles == 1 ? 4LL : 3LL) * current_sm_count();
+    p->min_span = 1;
+    p->spans = static_cast<int>(per_item == 0 || per_item * items > resident ? resident : per_item * items);
+    // workspace: unfinished pieces, then what an accumulating call leaves for its last launch
+    const size_t partials = round_up(static_cast<size_t>(2) * p->spans * rq::block_attention_slot_floats(a->cache.head_dim, p->query_tiles) * sizeof(float), 256);
+    const size_t lse = p->accumulate ? round_up(static_cast<size_t>(a->num_rows) * a->heads * sizeof(float), 256) : 0;
+    p->score_stride = (static_cast<int64_t>(p->max_len) + 7) / 8 * 8;
+    const size_t scores = p->accumulate ? round_up(static_cast<size_t>(a->num_rows) * a->heads * p->score_stride * sizeof(float), 256) : 0;
+    *workspace = partials + lse + scores;
+    p->partials = static_cast<float*>(a->workspace);
+    if (p->accumulate && a->workspace != nullptr) {
+        p->row_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + partials);
+        p->scores = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + partials + lse);
+    }
     return RQ_OK;
 }
 
@@ -748,7 +768,6 @@ int32_t rq_block_attention(const RqBlockAttentionArgs* a) {
     if (a->num_rows == 0) return RQ_OK;
     if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < need)
         return fail(RQ_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu", need, a->workspace_bytes);
-    p.row_lse = static_cast<float*>(a->workspace);
     p.programmatic_launch = chained(a->flags);
     const cudaError_t err = rq::launch_block_attention(p, a->cache.head_dim, a->cache.element == RQ_BLOCK_INT8, static_cast<cudaStream_t>(a->stream));
     return err == cudaSuccess ? RQ_OK : fail_cuda(err, "block attention launch");

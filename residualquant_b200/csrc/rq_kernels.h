@@ -155,9 +155,16 @@ struct BlockAttentionParams {
     int max_len;             // tokens from here on are not seen
     float scale_log2;        // softmax scale * log2(e)
     float* lse;              // or nullptr
-    float* row_lse;          // workspace [num_rows][heads]: log2 of the softmax denominator (accumulate)
+    int query_tiles;         // eights of queries that a CTA takes together
+    int spans, min_span;     // CTAs that the work is cut for, and the fewest chunks each takes
+    float* partials;         // workspace [2 * spans][8 * query_tiles][head_dim + 4]: value sums, m, l, M of unfinished pieces
+    float* scores;           // workspace [num_rows][heads][score_stride]: scores times log2(e) (accumulate), or nullptr
+    float* row_lse;          // workspace [num_rows][heads]: log2 of the softmax denominators (accumulate), or nullptr
+    int64_t score_stride;
     int programmatic_launch;
 };
+int block_attention_chunk();  // tokens that spans are counted in
+int block_attention_slot_floats(int head_dim, int query_tiles);
 cudaError_t launch_block_attention(const BlockAttentionParams& p, int head_dim, int int8, cudaStream_t stream);
 
 struct BlockEvictParams {
