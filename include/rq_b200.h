@@ -312,7 +312,7 @@ typedef enum RqActivation { RQ_ACTIVATION_BF16 = 0, RQ_ACTIVATION_FP16 = 1 } RqA
 typedef struct RqBlockCache {
     void* codes;   /* 16-byte aligned */
     float* scales;
-    float* weights; /* or NULL */
+    float* weights; /* 16-byte aligned, or NULL */
     int64_t num_blocks;
     int32_t kv_heads;
     int32_t head_dim;    /* 64, 96 or 128 */
@@ -378,6 +378,9 @@ typedef struct RqBlockAttentionArgs {
  * the arguments are not valid. */
 size_t rq_block_attention_workspace_bytes(const RqBlockAttentionArgs* args);
 int32_t rq_block_attention(const RqBlockAttentionArgs* args);
+/* Synchronizes `stream`: RQ_OK, or RQ_ERR_DEVICE_TIMEOUT if a bounded wait inside a block attention kernel ever gave up
+ * on the current device since the process began (that call's outputs are undefined). */
+int32_t rq_block_attention_status(void* stream);
 
 /* Bring every request of more than `budget` tokens down to `budget`: for each KV head on its own keep the first `sinks`
  * tokens, the last `recent` ones, and of the others those with the largest accumulated weight (ties: the lowest position;

@@ -47,6 +47,7 @@ EXPORTS = (
     "rq_block_append",
     "rq_block_attention",
     "rq_block_attention_workspace_bytes",
+    "rq_block_attention_status",
     "rq_block_evict",
     "rq_last_error",
     "rq_version",
@@ -282,6 +283,8 @@ def load() -> ctypes.CDLL:
     lib.rq_block_attention.restype = ctypes.c_int32
     lib.rq_block_attention_workspace_bytes.argtypes = [ctypes.POINTER(RqBlockAttentionArgs)]
     lib.rq_block_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.rq_block_attention_status.argtypes = [ctypes.c_void_p]
+    lib.rq_block_attention_status.restype = ctypes.c_int32
     lib.rq_block_evict.argtypes = [ctypes.POINTER(RqBlockEvictArgs)]
     lib.rq_block_evict.restype = ctypes.c_int32
     lib.rq_last_error.argtypes = []

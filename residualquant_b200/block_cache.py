@@ -59,7 +59,7 @@ class BlockCache:
         _require(
             weights is None
             or (weights.device == codes.device and weights.dtype == torch.float32 and weights.is_contiguous()
-                and tuple(weights.shape) == (blocks, heads, block_size)),
+                and weights.data_ptr() % 16 == 0 and tuple(weights.shape) == (blocks, heads, block_size)),
             "Contiguous FP32 [blocks, heads, block size] weights on the codes' device required",
         )
         self.codes, self.scales, self.weights = codes, scales, weights
@@ -171,6 +171,11 @@ class BlockCache:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
         self._call(self._lib.rq_block_attention, args)
+
+    def attention_status(self) -> None:
+        """Synchronize and raise if a bounded wait inside an attention kernel of any block cache ever gave up on this device."""
+        with torch.cuda.device(self.device):
+            _lib.check(self._lib.rq_block_attention_status(torch.cuda.current_stream().cuda_stream))
 
     def evict(self, seq_lens: torch.Tensor, block_table: torch.Tensor, budget: int, *, sinks: int = 0, recent: int = 0,
               kept: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -16,42 +16,61 @@
 // 2^15, exact to 2^-31 of the largest one below that).  Separate references for l and O keep blocks of tiny value scales
 // from losing either.
 //
-// Memory bound: 2 D bytes for each cached token and KV head.  All items' tokens, in units of kChunk, are laid end to end and
-// cut into equal spans, one for each CTA (four per SM, all resident), whatever the lengths are; the spans are found on the
-// device from the lengths, so that a captured launch stays right.  A span that ends inside an item leaves (m, l, M, O) in
-// the workspace, and a second launch joins those.  Each warp streams its own 16-token units through a ring of cp.async stages.
+// Memory bound: 2 D bytes for each cached token and KV head.  All items' tokens, in chunks of kChunk and kItemCost chunks
+// more for each item, are laid end to end and cut into equal spans, one for each CTA (four per SM, three with sixteen queries, all resident), whatever
+// the lengths are; the spans are found on the device from the lengths, so that a captured launch stays right.  A span that
+// ends inside an item leaves (m, l, M, O) in the workspace, and a second launch joins those.  Each warp streams its own
+// 16-token units through a ring of cp.async stages, and the next item's first units are set off before the warps join the
+// results of this one.
+#include <cuda.h>
+
 #include <algorithm>
 #include <atomic>
 
 #include "rq_block_common.cuh"
 
 namespace rq {
+
+__device__ int g_block_attention_status;
+
+struct AttentionLaunch {
+    alignas(64) CUtensorMap map;  // the codes as [2 * blocks][heads * page tokens][channels]
+    BlockAttentionParams p;
+};
+
 namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;              // tokens of one mma step
 constexpr int kChunk = kWarps * kUnit; // tokens that spans are counted in
-constexpr int kStages = 3;
+constexpr int kItemCost = 3;           // chunks' worth of time that a CTA spends on beginning and ending an item
+constexpr int resident(int query_tiles) { return query_tiles == 1 ? 4 : 3; }  // CTAs on a multiprocessor: registers for four or three
+constexpr int kJoinWarps = 8;
+constexpr uint32_t kWaitLimit = 1u << 22;  // polls of a copy's barrier before the kernel gives up
 constexpr float kNever = -1e30f;       // reference of a query that has seen no token
 constexpr float kSlack = 8.f;          // a reference is raised when exceeded by this many binades
 constexpr float kLift = 7.f;           // softmax weights are held times 2^kLift: at most 2^15 in fp16
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D_, bool INT8_, int NT_>
+template <int D_, bool INT8_, int NT_, bool SCORES_>
 struct Config {
     static constexpr int D = D_, NT = NT_;
     static constexpr bool kInt8 = INT8_;
+    static constexpr bool kScores = SCORES_;          // the scores are left behind, for the accumulated weights
     static constexpr int kRows = 8 * NT;              // queries of an item
     static constexpr int kSteps = D / 16;             // k16 steps of a score, and 16-channel tiles of an output
-    static constexpr int kPlane = D == 96 ? kUnit * 112 : kUnit * D;  // bytes of one plane of a unit in shared memory
+    static constexpr int kPlane = kUnit * D;          // bytes of one plane of a unit
     static constexpr int kStage = 2 * kPlane;
-    static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kMerge = kWarps * kRows * D * 4;
-    static constexpr int kArea = kRing > kMerge ? kRing : kMerge;     // the ring doubles as the warps' merge area
-    static constexpr int kOffInfo = kArea;                            // float4 [warps][stages]: K scale, log2 V scale, tokens
-    static constexpr int kOffStat = kOffInfo + kWarps * kStages * 16; // float [warps][rows][4]: m, l, M
-    static constexpr int kSmem = kOffStat + kWarps * kRows * 16;
+    // units in flight, the one in use included; its stage is where the warp's sums for eight queries go in the end
+    static constexpr int kStages = (D == 64 ? 6 : 3) + (NT == 1 ? 0 : 1);
+    static_assert(8 * D * 4 <= kStage, "a warp's sums fit a stage");
+    static constexpr int kOffInfo = kWarps * kStages * kStage;        // float4 [warps][stages]: K scale, log2 of V's, tokens
+    static constexpr int kOffStat = kOffInfo + kWarps * kStages * 16; // float [warps][8][4]: m, l, M, the stage of the sums
+    static constexpr int kOffQuery = kOffStat + kWarps * 8 * 16;      // 16-bit [rows][D]: the next piece's queries
+    static constexpr int kOffBarrier = kOffQuery + kRows * D * 2;     // uint64 [warps][stages]
+    static constexpr int kOffPlace = kOffBarrier + kWarps * kStages * 8;
+    static constexpr int kSmem = kOffPlace + 64;
     static constexpr int kSlot = D + 4;                               // floats a query's partial result takes
 };
 
@@ -66,16 +85,26 @@ __device__ __forceinline__ float log2_fast(float x) {
     return y;
 }
 
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool real) {
+__device__ __forceinline__ void copy16_or_zero(uint32_t to, const void* from, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
-}
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void wait_copies() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ void barrier_init(uint32_t barrier) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(barrier) : "memory"); }
+__device__ __forceinline__ void barrier_expect(uint32_t barrier, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool barrier_done(uint32_t barrier, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
+    return done != 0;
+}
+// kUnit tokens of a head from one page, rows row .. row + 15 of block `block` of the map.
+__device__ __forceinline__ void copy_unit(uint32_t to, const CUtensorMap* map, int row, int block, uint32_t barrier) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(to), "l"(map), "r"(0), "r"(row), "r"(block), "r"(barrier) : "memory");
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -106,14 +135,15 @@ __device__ __forceinline__ void to_half(uint32_t word, uint32_t& low, uint32_t& 
     }
 }
 
-// Where 16-byte piece `piece` of token `token` stands in a plane of a stage: rows of 128 bytes, pieces rotated by xor so
-// that the reads of eight rows (K) and of eight pieces of every second row (V) meet no bank twice; 64-byte rows go in pairs;
-// 96-byte rows are padded to 112, which does the same for 4-byte reads.
+// Where 16-byte piece `piece` of token `token` stands in a plane of a stage.  128-byte rows have their pieces rotated by xor
+// with the token (the copy's 128-byte swizzle), so that the reads of eight rows (K) and of eight pieces of every second row (V)
+// meet no bank twice; 64-byte rows the same by pairs (K's reads meet none, V's two); 96-byte rows are packed, and K's 8-byte
+// reads meet none, V's 4-byte ones two.
 template <int D>
 __device__ __forceinline__ int place(int token, int piece) {
     if constexpr (D == 128) return token * 128 + ((piece ^ (token & 7)) << 4);
-    if constexpr (D == 96) return token * 112 + (piece << 4);
-    return (token >> 1) * 128 + (((((token & 1) << 2) | piece) ^ (((token >> 1) & 3) << 1)) << 4);
+    if constexpr (D == 96) return token * 96 + (piece << 4);
+    return token * 64 + ((piece ^ ((token >> 1) & 3)) << 4);
 }
 
 // The work of request r: queries (rows x group), visible tokens, and its share of the chunk list.
@@ -123,36 +153,40 @@ struct Request {
     int tiles, chunks;
 };
 template <int ROWS>
-__device__ __forceinline__ Request request_of(const BlockAttentionParams& p, int r) {
+__device__ __forceinline__ Request request_from(const BlockAttentionParams& p, int first, int last, int length) {
     Request q;
-    q.first = p.v.query_start_loc[r];
-    const int last = p.v.query_start_loc[r + 1], length = p.v.seq_lens[r];
-    const int rows = max(0, min(last, p.num_rows) - q.first);
-    q.queries = rows * p.group;
+    q.first = first;
+    q.queries = max(0, min(last, p.num_rows) - first) * p.group;
     q.tokens = max(0, min(length, p.max_len));
-    q.before = length - (last - q.first);
+    q.before = length - (last - first);
     q.tiles = (q.queries + ROWS - 1) / ROWS;
     q.chunks = max(1, (q.tokens + kChunk - 1) / kChunk);
     return q;
 }
+template <int ROWS>
+__device__ __forceinline__ Request request_of(const BlockAttentionParams& p, int r) {
+    return request_from<ROWS>(p, p.v.query_start_loc[r], p.v.query_start_loc[r + 1], p.v.seq_lens[r]);
+}
 __device__ __forceinline__ int64_t work_of(const BlockAttentionParams& p, const Request& q) {
-    return static_cast<int64_t>(q.tiles) * p.v.kv_heads * q.chunks;
+    return static_cast<int64_t>(q.tiles) * p.v.kv_heads * (q.chunks + kItemCost);
 }
 
-// Sum of all requests' work, and the sum of those before request `until`, or (until < 0) the request that chunk `at * span`
-// falls into and the work before it.  All threads of the block take part.
+// Where things stand in the list of all items: each takes kItemCost units and one for each chunk, and the list is cut into
+// spans.  Finds the sum of all requests' units, and the request that span `at` begins in with the units before it.  All
+// threads of the block take part.
 struct Place {
     int64_t total, before, span;
     int request;
 };
+template <int WARPS>
 struct PlaceShared {
-    int64_t warp_sums[kWarps];
+    int64_t warp_sums[WARPS];
     int64_t before;
     int request;
 };
-template <int ROWS>
-__device__ __forceinline__ Place find_place(const BlockAttentionParams& p, PlaceShared& shared, int at, int until) {
-    const int n = p.v.num_requests, each = (n + kThreads - 1) / kThreads;
+template <int ROWS, int WARPS>
+__device__ __forceinline__ Place find_place(const BlockAttentionParams& p, PlaceShared<WARPS>& shared, int at) {
+    const int n = p.v.num_requests, each = (n + WARPS * 32 - 1) / (WARPS * 32);
     const int lo = min(n, static_cast<int>(threadIdx.x) * each), hi = min(n, lo + each);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int64_t sum = 0;
@@ -169,17 +203,16 @@ __device__ __forceinline__ Place find_place(const BlockAttentionParams& p, Place
     place.total = 0;
     int64_t running = inclusive - sum;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
         if (w < warp) running += shared.warp_sums[w];
         place.total += shared.warp_sums[w];
     }
     place.span = max(static_cast<int64_t>(p.min_span), (place.total + p.spans - 1) / p.spans);
     const int64_t target = at * place.span;
-    const bool mine = until < 0 ? (running <= target && target < running + sum) : (lo <= until && until < hi);
-    if (mine) {
+    if (running <= target && target < running + sum) {
         for (int r = lo; r < hi; ++r) {
-            const int64_t one = work_of(p, request_of<ROWS>(p, r));
-            if (until < 0 ? target < running + one : r == until) {
+            const int64_t one = each == 1 ? sum : work_of(p, request_of<ROWS>(p, r));
+            if (target < running + one) {
                 shared.before = running;
                 shared.request = r;
                 break;
@@ -209,98 +242,156 @@ __device__ __forceinline__ void write_output(const BlockAttentionParams& p, int 
 }
 
 template <typename C>
-__global__ void __launch_bounds__(kThreads, C::NT == 1 ? 4 : 3) block_attention_kernel(const BlockAttentionParams p) {
-    constexpr int D = C::D, NT = C::NT, kRows = C::kRows, kSteps = C::kSteps;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ PlaceShared place_shared;
+__global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_kernel(const __grid_constant__ AttentionLaunch launch) {
+    const BlockAttentionParams& p = launch.p;
+    constexpr int D = C::D, NT = C::NT, kRows = C::kRows, kSteps = C::kSteps, kStages = C::kStages;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    static_assert(sizeof(PlaceShared<kWarps>) <= 64, "room for the place");
+    PlaceShared<kWarps>& place_shared = *reinterpret_cast<PlaceShared<kWarps>*>(smem + C::kOffPlace);
     const BlockView& v = p.v;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int page_shift = v.page_tokens == 16 ? 4 : 5;
     pdl_wait();
     pdl_launch_dependents();
-    const Place start = find_place<kRows>(p, place_shared, blockIdx.x, -1);
-    int64_t at = blockIdx.x * start.span;
-    const int64_t end = min(at + start.span, start.total);
-    if (at >= end) return;
-    int r = start.request;
-    int64_t before = start.before;  // work ahead of request r
-    Request q = request_of<kRows>(p, r);
-    const int64_t plane_bytes = v.num_blocks * v.kv_heads * static_cast<int64_t>(v.page_tokens) * D;
+    const Place start = find_place<kRows, kWarps>(p, place_shared, blockIdx.x);
+    const int64_t begin = blockIdx.x * start.span, end = min(begin + start.span, start.total);
+    if (tid == 0) p.cuts[blockIdx.x].pieces = 0;  // until an item is found that goes on in the next span
+    if (begin >= end) return;
     const int64_t plane_scales = v.num_blocks * v.kv_heads;
     uint8_t* ring = smem + warp * kStages * C::kStage;
     const uint32_t ring_address = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
     float4* info = reinterpret_cast<float4*>(smem + C::kOffInfo) + warp * kStages;
     float* stats = reinterpret_cast<float*>(smem + C::kOffStat);
+    const uint32_t barriers = static_cast<uint32_t>(__cvta_generic_to_shared(smem + C::kOffBarrier)) + warp * kStages * 8;
+    if (lane < kStages) barrier_init(barriers + lane * 8);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the barriers are there for the copies
+    __syncwarp();
+    uint32_t phases = 0u;  // bit s: parity of the copy into stage s that is waited for next
 
-    while (at < end) {
-        int64_t local = at - before;
-        if (local >= work_of(p, q)) {  // on to the next request that has work (there is one: at < total)
-            before += work_of(p, q);
-            q = request_of<kRows>(p, ++r);
-            continue;
-        }
-        const int item = static_cast<int>(local / q.chunks);
-        const int chunk0 = static_cast<int>(local - static_cast<int64_t>(item) * q.chunks);
-        const int chunk1 = static_cast<int>(min(static_cast<int64_t>(q.chunks), chunk0 + (end - at)));
-        const int head = item % v.kv_heads, query0 = item / v.kv_heads * kRows;
-        const int token_begin = chunk0 * kChunk, token_end = min(chunk1 * kChunk, q.tokens);
-        const int all_units = (token_end - token_begin + kUnit - 1) / kUnit;
-        const int units = all_units > warp ? (all_units - warp + kWarps - 1) / kWarps : 0;
-
-        // page ids: lane i holds that of the warp's unit 32 w + i, one window ahead
-        const int32_t* table = v.block_table + static_cast<int64_t>(r) * v.table_stride;
-        auto window = [&](int first) {
-            const int unit = first + lane;
-            return unit < units ? table[(token_begin + (warp + unit * kWarps) * kUnit) >> page_shift] : -1;
-        };
-        int ids = window(0), ids_next = units > 32 ? window(32) : -1;
-        auto produce = [&](int unit, int stage) {
-            if (unit < units) {
-                if ((unit & 31) == 0 && unit > 0) {
-                    ids = ids_next;
-                    ids_next = window(unit + 32);
-                }
-                const int id = __shfl_sync(kFullMask, ids, unit & 31);
-                const int token0 = token_begin + (warp + unit * kWarps) * kUnit;
-                const bool real = id >= 0 && id < v.num_blocks;
-                const int count = real ? min(kUnit, token_end - token0) : 0;  // the rest is zero-filled
-                const int64_t page = real ? static_cast<int64_t>(id) * v.kv_heads + head : 0;
-                const uint8_t* from = v.codes + ((page << page_shift) + (token0 & (v.page_tokens - 1))) * D;
-                const uint32_t to = ring_address + stage * C::kStage;
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const int piece = i * 32 + lane, token = piece / (D / 16);
-                    const int offset = place<D>(token, piece % (D / 16));
-                    const bool in = token < count;
-                    copy16(to + offset, from + piece * 16, in);
-                    copy16(to + C::kPlane + offset, from + plane_bytes + piece * 16, in);
-                }
-                float* word = reinterpret_cast<float*>(info + stage);
-                if (lane < 2) copy4(static_cast<uint32_t>(__cvta_generic_to_shared(word + lane)), v.scales + lane * plane_scales + page);
-                if (lane == 2) word[2] = __int_as_float(count);
+    // The span's pieces, one after the other; all of this but `units` is the same in every thread of the block.
+    int64_t at = begin;
+    int r = start.request;
+    int64_t ahead = start.before;  // units of work ahead of request r
+    Request q = request_of<kRows>(p, r);
+    int head, query0, token_begin, token_end;
+    int units;           // of the piece, this warp's
+    bool whole;          // the piece is all of its item
+    int more_spans;      // the piece begins its item: spans behind this one that go on with it
+    int64_t slot;        // else: where its result goes
+    // Windows: lane i holds the page id of the warp's unit 32 w + i (-1: none, or outside the cache) and its scales, and of
+    // the window after it the ids from the window's start on and the scales from its middle on.
+    int ids, ids_next;
+    float key_scales, value_scales, key_scales_next, value_scales_next;  // the latter as log2
+    auto window = [&](int first) {
+        const int unit = first + lane;
+        const int id = unit < units ? v.block_table[static_cast<int64_t>(r) * v.table_stride + ((token_begin + (warp + unit * kWarps) * kUnit) >> page_shift)] : -1;
+        return id < v.num_blocks ? id : -1;
+    };
+    auto scale = [&](int id, int plane) { return id >= 0 ? v.scales[plane * plane_scales + static_cast<int64_t>(id) * v.kv_heads + head] : 1.f; };
+    auto next_piece = [&]() -> bool {
+        while (at < end) {
+            const int64_t local = at - ahead;
+            if (local >= work_of(p, q)) {  // on to the next request that has work (there is one: at < total)
+                ahead += work_of(p, q);
+                q = request_of<kRows>(p, ++r);
+                continue;
             }
-            commit_copies();
-        };
+            const int cost = q.chunks + kItemCost;
+            const int item = static_cast<int>(local / cost), done = static_cast<int>(local - static_cast<int64_t>(item) * cost);
+            const int upto = static_cast<int>(min(static_cast<int64_t>(cost), done + (end - at)));
+            const int chunk0 = max(0, done - kItemCost), chunk1 = upto - kItemCost;
+            // a span leaves at most two unfinished pieces: one that goes on at its start, and one that begins inside it
+            slot = 2LL * blockIdx.x + (at == begin && done >= kItemCost ? 0 : 1);
+            at += upto - done;
+            if (chunk1 <= chunk0) continue;  // the span ends before the item's first chunk
+            whole = chunk0 == 0 && chunk1 == q.chunks;
+            more_spans = chunk0 == 0 && !whole ? static_cast<int>((ahead + static_cast<int64_t>(item + 1) * cost - 1) / start.span) - static_cast<int>(blockIdx.x) : 0;
+            head = item % v.kv_heads;
+            query0 = item / v.kv_heads * kRows;
+            token_begin = chunk0 * kChunk;
+            token_end = min(chunk1 * kChunk, q.tokens);
+            const int all_units = (token_end - token_begin + kUnit - 1) / kUnit;
+            units = all_units > warp ? (all_units - warp + kWarps - 1) / kWarps : 0;
+            ids = window(0);
+            ids_next = window(32);
+            return true;
+        }
+        return false;
+    };
+    // Sets the copies of a unit off, and says what the unit is.
+    auto produce = [&](int unit, int to) {
+        if (unit >= units) return;
+        if ((unit & 31) == 0 && unit > 0) {
+            ids = ids_next;
+            ids_next = window(unit + 32);
+            key_scales = key_scales_next;
+            value_scales = value_scales_next;
+        }
+        const int id = __shfl_sync(kFullMask, ids, unit & 31);
+        const int token0 = token_begin + (warp + unit * kWarps) * kUnit;
+        if (lane == 0) {
+            const uint32_t barrier = barriers + to * 8;
+            barrier_expect(barrier, id >= 0 ? C::kStage : 0);
+            if (id >= 0) {
+                const int row = (head << page_shift) + (token0 & (v.page_tokens - 1));
+                copy_unit(ring_address + to * C::kStage, &launch.map, row, id, barrier);
+                copy_unit(ring_address + to * C::kStage + C::kPlane, &launch.map, row, static_cast<int>(v.num_blocks) + id, barrier);
+            }
+        }
+        if ((unit & 31) == 0) {
+            if (unit == 0) {
+                key_scales = scale(ids, 0);
+                value_scales = log2_fast(scale(ids, 1));
+            }
+        } else if ((unit & 31) == 16) {
+            key_scales_next = scale(ids_next, 0);
+            value_scales_next = log2_fast(scale(ids_next, 1));
+        }
+    };
+    auto describe = [&](int unit, int to) {
+        if (unit >= units) return;
+        const int id = __shfl_sync(kFullMask, ids, unit & 31);
+        const float k = __shfl_sync(kFullMask, key_scales, unit & 31), log_v = __shfl_sync(kFullMask, value_scales, unit & 31);
+        const int count = id >= 0 ? min(kUnit, token_end - (token_begin + (warp + unit * kWarps) * kUnit)) : 0;
+        if (lane == 0) info[to] = make_float4(k, log_v, __int_as_float(count), 0.f);
+    };
+    int stage = 0;       // of the next unit to be used
+    auto set_off = [&]() {
+        // the piece's queries, ahead of the queue of cache copies (rows behind the item's last are zeros)
+        for (int i = tid; i < kRows * (D / 8); i += kThreads) {
+            const int query = query0 + i / (D / 8);
+            const bool real = query < q.queries;
+            const int row = real ? q.first + query / p.group : q.first, query_head = head * p.group + (real ? query % p.group : 0);
+            copy16_or_zero(static_cast<uint32_t>(__cvta_generic_to_shared(smem + C::kOffQuery + i * 16)),
+                           static_cast<const uint16_t*>(p.query) + row * p.query_stride + query_head * D + i % (D / 8) * 8, real);
+        }
+        commit_copies();
+        // the piece's first units, into the ring but for the stage that is free
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) produce(i, i);
+        for (int i = 0; i < kStages - 1; ++i) produce(i, stage + i < kStages ? stage + i : stage + i - kStages);
+    };
+    bool failed = false;
+    bool more = next_piece();
+    if (more) {
+        set_off();
+        wait_copies();
+        __syncthreads();
+    }
 
-        // this thread's query channels as fp16: query 8 n + g, the channels that its K words hold
+    while (more) {
+        // the queries as fp16
         uint32_t qf[NT][kSteps][2];
         float factor[NT][2];   // score units of queries 8 n + 2 t + {0, 1}
         int limit[NT][2];      // tokens that they see
         int least = 0x7fffffff;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int query = query0 + n * 8 + g;
-            const bool real = query < q.queries;
-            const int row = q.first + query / p.group, query_head = head * p.group + query % p.group;
-            const uint16_t* from = static_cast<const uint16_t*>(p.query) + row * p.query_stride + query_head * D;
+            // query 8 n + g, the channels that this thread's K words hold: four of step s, inside its D / 4 contiguous ones
             uint32_t raw[kSteps][2];
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                // channels of step s: four of them, at 16 s + 4 t (D = 96) or inside this thread's D / 4 contiguous ones
-                const int channel = D == 96 ? s * 16 + t * 4 : t * (D / 4) + s * 4;
-                const uint2 two = real ? *reinterpret_cast<const uint2*>(from + channel) : make_uint2(0u, 0u);
+                const int channel = t * (D / 4) + s * 4;
+                const uint2 two = *reinterpret_cast<const uint2*>(smem + C::kOffQuery + ((n * 8 + g) * D + channel) * 2);
                 raw[s][0] = two.x;
                 raw[s][1] = two.y;
             }
@@ -336,6 +427,18 @@ __global__ void __launch_bounds__(kThreads, C::NT == 1 ? 4 : 3) block_attention_
             }
         }
         least = __reduce_min_sync(kFullMask, least);
+        float* score_at[NT][2];
+        if constexpr (C::kScores) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int column = query0 + n * 8 + 2 * t + i;
+                    const int64_t query_row = static_cast<int64_t>(q.first + column / p.group) * p.heads + head * p.group + column % p.group;
+                    score_at[n][i] = column < q.queries ? p.scores + query_row * p.score_stride : nullptr;
+                }
+            }
+        }
 
         float o[kSteps][NT][4];
         float m[NT][2], M[NT][2], l[NT][2];
@@ -350,23 +453,30 @@ __global__ void __launch_bounds__(kThreads, C::NT == 1 ? 4 : 3) block_attention_
             for (int s = 0; s < kSteps; ++s) o[s][n][0] = o[s][n][1] = o[s][n][2] = o[s][n][3] = 0.f;
         }
 
-        int stage = 0, next = kStages - 1;
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) describe(i, stage + i < kStages ? stage + i : stage + i - kStages);
         for (int unit = 0; unit < units; ++unit) {
-            wait_copies<kStages - 2>();
-            __syncwarp();
-            produce(unit + kStages - 1, next);
+            const int free_stage = stage == 0 ? kStages - 1 : stage - 1;  // the one that the unit before was in
+            __syncwarp();                                                 // no lane reads it any more
+            produce(unit + kStages - 1, free_stage);
+            describe(unit + kStages - 1, free_stage);
+            uint32_t polls = 0;
+            while (!barrier_done(barriers + stage * 8, phases >> stage & 1u) && !failed) failed = ++polls > kWaitLimit;
+            phases ^= 1u << stage;
             const uint8_t* keys = ring + stage * C::kStage;
             const uint8_t* values = keys + C::kPlane;
             const float4 about = info[stage];
-            next = stage;
             stage = stage + 1 == kStages ? 0 : stage + 1;
             const int token0 = token_begin + (warp + unit * kWarps) * kUnit;
             const int count = __float_as_int(about.z);
 
             // scores
-            float x[NT][4];
+            float x[NT][4], x_odd[NT][4];  // two sums, so that half the products wait for one another
 #pragma unroll
-            for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[n][i] = x_odd[n][i] = 0.f;
+            }
             uint32_t low[kSteps], high[kSteps];  // K words of tokens g and g + 8
             if constexpr (D == 128) {
 #pragma unroll
@@ -384,8 +494,11 @@ __global__ void __launch_bounds__(kThreads, C::NT == 1 ? 4 : 3) block_attention_
             } else {
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
-                    low[s] = *reinterpret_cast<const uint32_t*>(keys + place<D>(g, s) + t * 4);
-                    high[s] = *reinterpret_cast<const uint32_t*>(keys + place<D>(g + 8, s) + t * 4);
+                    if (s & 1) continue;
+                    const uint2 a = *reinterpret_cast<const uint2*>(keys + g * 96 + t * 24 + s * 4);
+                    const uint2 b = *reinterpret_cast<const uint2*>(keys + (g + 8) * 96 + t * 24 + s * 4);
+                    low[s] = a.x; low[s + 1] = a.y;
+                    high[s] = b.x; high[s + 1] = b.y;
                 }
             }
 #pragma unroll
@@ -394,16 +507,16 @@ __global__ void __launch_bounds__(kThreads, C::NT == 1 ? 4 : 3) block_attention_
                 to_half<C::kInt8>(low[s], a[0], a[2]);
                 to_half<C::kInt8>(high[s], a[1], a[3]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma(x[n], a, qf[n][s][0], qf[n][s][1]);
+                for (int n = 0; n < NT; ++n) mma(s & 1 ? x_odd[n] : x[n], a, qf[n][s][0], qf[n][s][1]);
             }
-            const float value_scale = log2_fast(about.y);
+            const float value_scale = about.y;
             const bool masked = count < kUnit || token0 + kUnit > least;
             bool raise = false;
             float top[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[n][i] *= about.x * factor[n][i & 1];
+                for (int i = 0; i < 4; ++i) x[n][i] = (x[n][i] + x_odd[n][i]) * (about.x * factor[n][i & 1]);
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -417,16 +530,13 @@ __global__ void __launch_bounds__(kThreads, C::NT == 1 ? 4 : 3) block_attention_
                     raise = raise || top[n][i] > m[n][i] + kSlack || top[n][i] + value_scale > M[n][i] + kSlack;
                 }
             }
-            if (p.scores != nullptr) {
+            if constexpr (C::kScores) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int column = query0 + n * 8 + 2 * t + (i & 1), token = token0 + g + (i >> 1) * 8;
-                        if (column < q.queries && token < limit[n][i & 1]) {
-                            const int row = q.first + column / p.group, query_head = head * p.group + column % p.group;
-                            p.scores[(static_cast<int64_t>(row) * p.heads + query_head) * p.score_stride + token] = x[n][i];
-                        }
+                        const int token = token0 + g + (i >> 1) * 8;
+                        if (score_at[n][i & 1] != nullptr && token < limit[n][i & 1]) score_at[n][i & 1][token] = x[n][i];
                     }
                 }
             }
@@ -478,7 +588,16 @@ __global__ void __launch_bounds__(kThreads, C::NT == 1 ? 4 : 3) block_attention_
                     word[i][0] = a.x; word[i][1] = a.y;
                 } else {
 #pragma unroll
-                    for (int w = 0; w < kWords; ++w) word[i][w] = *reinterpret_cast<const uint32_t*>(values + token * 112 + g * 12 + w * 4);
+                    for (int w = 0; w < kWords; ++w) word[i][w] = *reinterpret_cast<const uint32_t*>(values + token * 96 + g * 12 + w * 4);
+                }
+            }
+            if (count < kUnit) {  // whatever stands behind the last token, a weight of 0 must not meet it
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (2 * t + (i & 1) + (i >> 1) * 8 >= count) {
+#pragma unroll
+                        for (int w = 0; w < kWords; ++w) word[i][w] = 0u;
+                    }
                 }
             }
 #pragma unroll
@@ -494,181 +613,239 @@ __global__ void __launch_bounds__(kThreads, C::NT == 1 ? 4 : 3) block_attention_
             }
         }
 
-        // ---- the warps' results are joined ----
-        wait_copies<0>();
-        __syncthreads();
-        float* area = reinterpret_cast<float*>(smem);
+        // ---- the warps' results are joined, while the next piece's units are on their way ----
+        const int done_first = q.first, done_queries = q.queries, done_head = head, done_query0 = query0;
+        const bool done_whole = whole;
+        if (more_spans > 0 && tid == 0) p.cuts[blockIdx.x] = {more_spans + 1, static_cast<int>(slot & 1), q.first, q.queries - query0, query0, head};
+        const int64_t done_slot = slot;
+        more = next_piece();
+        if (more) set_off();
+        const int last = stage == 0 ? kStages - 1 : stage - 1;  // the stage that is free
+        float* area = reinterpret_cast<float*>(ring + last * C::kStage);
+        __syncwarp();  // no lane reads the last unit any more
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int step = 4; step < 32; step <<= 1) l[n][i] += __shfl_xor_sync(kFullMask, l[n][i], step);
-                const int column = n * 8 + 2 * t + i;
-                float* to = area + (warp * kRows + column) * D + g * (D / 8);
+                const int column = 2 * t + i;
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) *reinterpret_cast<float2*>(to + 2 * s) = make_float2(o[s][n][i], o[s][n][i + 2]);
-                if (g == 0) *reinterpret_cast<float4*>(stats + (warp * kRows + column) * 4) = make_float4(m[n][i], l[n][i], M[n][i], 0.f);
+                for (int s = 0; s < kSteps; ++s)
+                    *reinterpret_cast<float2*>(area + column * D + g * (D / 8) + 2 * s) = make_float2(o[s][n][i], o[s][n][i + 2]);
+                if (g == 0)
+                    *reinterpret_cast<float4*>(stats + (warp * 8 + column) * 4) = make_float4(m[n][i], l[n][i], M[n][i], __int_as_float(last));
             }
+            __syncthreads();
+            for (int piece = tid; piece < 8 * (D / 4); piece += kThreads) {
+                const int column = piece / (D / 4), channel = piece % (D / 4) * 4;
+                const int query = done_query0 + n * 8 + column;
+                if (query >= done_queries) continue;
+                float4 stat[kWarps];
+                float m_all = kNever, M_all = kNever, l_all = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    stat[w] = *reinterpret_cast<const float4*>(stats + (w * 8 + column) * 4);
+                    m_all = fmaxf(m_all, stat[w].x);
+                    M_all = fmaxf(M_all, stat[w].z);
+                }
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float4 part = *reinterpret_cast<const float4*>(smem + (w * kStages + __float_as_int(stat[w].w)) * C::kStage + (column * D + channel) * 4);
+                    const float share = exp2_fast(stat[w].z - M_all);
+                    l_all += stat[w].y * exp2_fast(stat[w].x - m_all);
+                    sum.x += part.x * share;
+                    sum.y += part.y * share;
+                    sum.z += part.z * share;
+                    sum.w += part.w * share;
+                }
+                if (done_whole) {
+                    write_output(p, done_first + query / p.group, done_head * p.group + query % p.group, D, channel, sum, m_all, l_all, M_all);
+                } else {
+                    float* to = p.partials + (done_slot * kRows + n * 8 + column) * C::kSlot;
+                    *reinterpret_cast<float4*>(to + channel) = sum;
+                    if (channel == 0) *reinterpret_cast<float4*>(to + D) = make_float4(m_all, l_all, M_all, 0.f);
+                }
+            }
+            if (n == NT - 1) {
+                wait_copies();                                                // the next piece's queries
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies into the sums' stages come after the sums
+            }
+            __syncthreads();  // the sums have been read: their stages are free
         }
-        __syncthreads();
-        const bool whole = chunk0 == 0 && chunk1 == q.chunks;
-        // a span leaves at most two unfinished pieces: the one at its start and the one at its end
-        const int64_t slot = 2LL * blockIdx.x + (at > blockIdx.x * start.span ? 1 : 0);
-        for (int piece = tid; piece < kRows * (D / 4); piece += kThreads) {
-            const int column = piece / (D / 4), channel = piece % (D / 4) * 4;
-            const int query = query0 + column;
-            if (query >= q.queries) continue;
-            float4 stat[kWarps];
-            float m_all = kNever, M_all = kNever, l_all = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                stat[w] = *reinterpret_cast<const float4*>(stats + (w * kRows + column) * 4);
-                m_all = fmaxf(m_all, stat[w].x);
-                M_all = fmaxf(M_all, stat[w].z);
-            }
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float4 part = *reinterpret_cast<const float4*>(area + (w * kRows + column) * D + channel);
-                const float share = exp2_fast(stat[w].z - M_all);
-                l_all += stat[w].y * exp2_fast(stat[w].x - m_all);
-                sum.x += part.x * share;
-                sum.y += part.y * share;
-                sum.z += part.z * share;
-                sum.w += part.w * share;
-            }
-            if (whole) {
-                write_output(p, q.first + query / p.group, head * p.group + query % p.group, D, channel, sum, m_all, l_all, M_all);
-            } else {
-                float* to = p.partials + (slot * kRows + column) * C::kSlot;
-                *reinterpret_cast<float4*>(to + channel) = sum;
-                if (channel == 0) *reinterpret_cast<float4*>(to + D) = make_float4(m_all, l_all, M_all, 0.f);
-            }
-        }
-        __syncthreads();
-        at += chunk1 - chunk0;
+    }
+    if (failed) {  // a copy did not arrive in time (no case is known): the call's results are not to be used
+        atomicExch(&g_block_attention_status, RQ_ERR_DEVICE_TIMEOUT);
+        for (uint32_t polls = 0; polls < kWaitLimit && !barrier_done(barriers + stage * 8, phases >> stage & 1u); ++polls) {}
     }
 }
 
-// Joins the pieces of the items that more than one span took part in: one CTA for each (row, query head).
+// Joins the pieces of the items that more than one span took part in.  At most one such item begins in a span; the CTAs of
+// row `part` of the grid take every gridDim.y-th of its queries, all of their warps on as few at a time as leave none out.
 template <typename C>
-__global__ void __launch_bounds__(kThreads) block_join_kernel(const BlockAttentionParams p) {
-    constexpr int D = C::D, kRows = C::kRows, kLanes = D / 4;
-    __shared__ PlaceShared place_shared;
-    __shared__ float4 sums[kWarps][kLanes];
-    __shared__ float2 totals[kWarps], tops[kWarps];
-    const BlockView& v = p.v;
+__global__ void __launch_bounds__(kJoinWarps * 32) block_join_kernel(const BlockAttentionParams p) {
+    constexpr int D = C::D, kRows = C::kRows, kLanes = D / 4, kBatch = 8;
+    __shared__ float4 sums[kJoinWarps][kLanes];
+    __shared__ float4 stats[kJoinWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int row = blockIdx.x / p.heads, query_head = blockIdx.x % p.heads, head = query_head / p.group;
     pdl_wait();
     pdl_launch_dependents();
-    const int r = find_request(v.query_start_loc, v.num_requests, row, lane);
-    if (r >= v.num_requests) return;
-    const Request q = request_of<kRows>(p, r);
-    if (row < q.first || q.chunks == 1) return;
-    const Place place = find_place<kRows>(p, place_shared, 0, r);
-    const int query = (row - q.first) * p.group + query_head % p.group, column = query % kRows;
-    const int64_t a = place.before + (static_cast<int64_t>(query / kRows) * v.kv_heads + head) * q.chunks, b = a + q.chunks;
-    const int first = static_cast<int>(a / place.span), count = static_cast<int>((b - 1) / place.span) - first + 1;
-    if (count == 1) return;
-    auto part = [&](int i) -> const float* {
-        const int64_t slot = 2LL * (first + i) + (i == 0 && a > first * place.span ? 1 : 0);
-        return p.partials + (slot * kRows + column) * C::kSlot;
-    };
-    float m = kNever, M = kNever;
-    for (int i = tid; i < count; i += kThreads) {
-        const float4 stat = *reinterpret_cast<const float4*>(part(i) + D);
-        m = fmaxf(m, stat.x);
-        M = fmaxf(M, stat.z);
-    }
+    const int each = (p.spans + gridDim.x - 1) / gridDim.x, behind = min(p.spans, static_cast<int>(blockIdx.x + 1) * each);
+    for (int span = blockIdx.x * each; span < behind; ++span) {
+        const BlockCut cut = p.cuts[span];
+        if (cut.pieces == 0) continue;
+        const int queries = min(kRows, cut.queries), parts = gridDim.y;
+        int together = 1;  // queries that the CTA works on at a time
+        while (together < kJoinWarps && together * parts < queries) together *= 2;
+        const int warps = kJoinWarps / together, mine = warp % warps;  // warps that share a query
+        for (int base = blockIdx.y * together; base < queries; base += parts * together) {
+            const int column = base + warp / warps;
+            float m = kNever, M = kNever, l = 0.f;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (column < queries) {
+                for (int first = mine; first < cut.pieces; first += warps * kBatch) {
+                    float4 stat[kBatch], x[kBatch];
+    #pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {  // (without branches, so that all loads are on their way at once)
+                        const int i = min(first + j * warps, cut.pieces - 1);
+                        const int64_t slot = 2LL * (span + i) + (i == 0 ? cut.inside : 0);
+                        const float* from = p.partials + (slot * kRows + column) * C::kSlot;
+                        stat[j] = __ldcg(reinterpret_cast<const float4*>(from + D));
+                        x[j] = __ldcg(reinterpret_cast<const float4*>(from + (lane < kLanes ? lane * 4 : 0)));
+                    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-        M = fmaxf(M, __shfl_xor_sync(kFullMask, M, o));
-    }
-    if (lane == 0) tops[warp] = make_float2(m, M);
-    __syncthreads();
+                    for (int j = 0; j < kBatch; ++j)
+                        if (first + j * warps >= cut.pieces) stat[j] = make_float4(kNever, 0.f, kNever, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        m = fmaxf(m, tops[w].x);
-        M = fmaxf(M, tops[w].y);
-    }
-    float l = 0.f;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = warp; i < count; i += kWarps) {
-        const float* from = part(i);
-        const float4 stat = *reinterpret_cast<const float4*>(from + D);
-        const float share = exp2_fast(stat.z - M);
-        l += stat.y * exp2_fast(stat.x - m);
-        if (lane < kLanes) {
-            const float4 x = *reinterpret_cast<const float4*>(from + lane * 4);
-            sum.x += x.x * share;
-            sum.y += x.y * share;
-            sum.z += x.z * share;
-            sum.w += x.w * share;
+                    for (int j = 0; j < kBatch; ++j) {
+                        const float m_new = fmaxf(m, stat[j].x), M_new = fmaxf(M, stat[j].z);
+                        l = l * exp2_fast(m - m_new) + stat[j].y * exp2_fast(stat[j].x - m_new);
+                        const float keep = exp2_fast(M - M_new), share = first + j * warps < cut.pieces ? exp2_fast(stat[j].z - M_new) : 0.f;
+                        sum.x = sum.x * keep + x[j].x * share;
+                        sum.y = sum.y * keep + x[j].y * share;
+                        sum.z = sum.z * keep + x[j].z * share;
+                        sum.w = sum.w * keep + x[j].w * share;
+                        m = m_new;
+                        M = M_new;
+                    }
+                }
+            }
+            if (warps > 1) {
+                if (lane < kLanes) sums[warp][lane] = sum;
+                if (lane == 0) stats[warp] = make_float4(m, l, M, 0.f);
+                __syncthreads();
+                if (mine == 0 && column < queries) {
+                    for (int w = 1; w < warps; ++w) {
+                        const float4 stat = stats[warp + w], x = sums[warp + w][lane < kLanes ? lane : 0];
+                        const float m_new = fmaxf(m, stat.x), M_new = fmaxf(M, stat.z);
+                        l = l * exp2_fast(m - m_new) + stat.y * exp2_fast(stat.x - m_new);
+                        const float keep = exp2_fast(M - M_new), share = exp2_fast(stat.z - M_new);
+                        sum.x = sum.x * keep + x.x * share;
+                        sum.y = sum.y * keep + x.y * share;
+                        sum.z = sum.z * keep + x.z * share;
+                        sum.w = sum.w * keep + x.w * share;
+                        m = m_new;
+                        M = M_new;
+                    }
+                }
+                __syncthreads();
+            }
+            if (mine == 0 && column < queries && lane < kLanes) {
+                const int query = cut.query0 + column;
+                write_output(p, cut.first + query / p.group, cut.head * p.group + query % p.group, D, lane * 4, sum, m, l, M);
+            }
         }
-    }
-    if (lane < kLanes) sums[warp][lane] = sum;
-    if (lane == 0) totals[warp] = make_float2(l, 0.f);
-    __syncthreads();
-    if (tid < kLanes) {
-        l = 0.f;
-        sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float4 x = sums[w][tid];
-            l += totals[w].x;
-            sum.x += x.x;
-            sum.y += x.y;
-            sum.z += x.z;
-            sum.w += x.w;
-        }
-        write_output(p, row, query_head, D, tid * 4, sum, m, l, M);
     }
 }
 
-// Adds 2^(score - lse), summed over the rows and query heads of a KV head, to the weights: one thread for each token.
-// One CTA adds to a token's weight in a call, so the sum's order is fixed; the atomic is for requests that share blocks.
+// Adds 2^(score - lse), summed over the rows and query heads of a KV head, to the weights: four tokens a thread.  One thread
+// adds to a token's weight in a call, so the sum's order is fixed; the atomic is for requests that share blocks.
 __global__ void __launch_bounds__(kThreads) block_weights_kernel(const BlockAttentionParams p) {
     const BlockView& v = p.v;
     const int r = blockIdx.x / v.kv_heads, head = blockIdx.x % v.kv_heads;
-    pdl_wait();
-    pdl_launch_dependents();
     const Request q = request_of<8>(p, r);
     const int page_shift = v.page_tokens == 16 ? 4 : 5;
-    for (int token = blockIdx.y * kThreads + threadIdx.x; token < q.tokens; token += gridDim.y * kThreads) {
-        const int id = v.block_table[static_cast<int64_t>(r) * v.table_stride + (token >> page_shift)];
-        if (id < 0 || id >= v.num_blocks) continue;
-        float sum = 0.f;
-        for (int query = 0; query < q.queries; ++query) {
-            if (token > q.before + query / p.group) continue;
-            const int64_t at = static_cast<int64_t>(q.first + query / p.group) * p.heads + head * p.group + query % p.group;
-            sum += exp2_fast(p.scores[at * p.score_stride + token] - p.row_lse[at]);
+    int token = (blockIdx.y * kThreads + threadIdx.x) * 4;
+    int id = token < q.tokens ? v.block_table[static_cast<int64_t>(r) * v.table_stride + (token >> page_shift)] : -1;
+    pdl_wait();
+    pdl_launch_dependents();
+    while (token < q.tokens) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // the first row that sees a token stands at the token's position, or is the request's first
+        const int first_row = max(0, token - q.before);
+        int64_t at = static_cast<int64_t>(q.first + first_row) * p.heads + head * p.group;
+        for (int row = first_row; row * p.group < q.queries; ++row, at += p.heads) {
+            const int seen = q.before + row + 1 - token;  // of the four
+#pragma unroll 4
+            for (int h = 0; h < p.group; ++h) {
+                const float4 x = *reinterpret_cast<const float4*>(p.scores + (at + h) * p.score_stride + token);
+                const float lse = p.row_lse[at + h];
+                sum[0] += exp2_fast(x.x - lse);
+                if (seen > 1) sum[1] += exp2_fast(x.y - lse);
+                if (seen > 2) sum[2] += exp2_fast(x.z - lse);
+                if (seen > 3) sum[3] += exp2_fast(x.w - lse);
+            }
         }
-        if (sum != 0.f) atomicAdd(v.weights + ((static_cast<int64_t>(id) * v.kv_heads + head) << page_shift) + (token & (v.page_tokens - 1)), sum);
+        if (id >= 0 && id < v.num_blocks) {
+            float* to = v.weights + ((static_cast<int64_t>(id) * v.kv_heads + head) << page_shift) + (token & (v.page_tokens - 1));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (token + i < q.tokens && sum[i] != 0.f) atomicAdd(to + i, sum[i]);
+        }
+        token += gridDim.y * kThreads * 4;
+        id = token < q.tokens ? v.block_table[static_cast<int64_t>(r) * v.table_stride + (token >> page_shift)] : -1;
     }
 }
 
-template <int D, bool INT8, int NT>
+// The tensor map of the codes: boxes of kUnit tokens of one head.
+cudaError_t describe_codes(const BlockView& v, int head_dim, CUtensorMap* map) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static std::atomic<Encode> known{nullptr};
+    Encode encode = known.load(std::memory_order_acquire);
+    if (encode == nullptr) {
+        void* found = nullptr;
+        cudaDriverEntryPointQueryResult status;
+        const cudaError_t err = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &found, 12000, cudaEnableDefault, &status);
+        if (err != cudaSuccess) return err;
+        if (status != cudaDriverEntryPointSuccess || found == nullptr) return cudaErrorNotSupported;
+        encode = reinterpret_cast<Encode>(found);
+        known.store(encode, std::memory_order_release);
+    }
+    const cuuint64_t rows = static_cast<cuuint64_t>(v.kv_heads) * v.page_tokens;
+    const cuuint64_t sizes[3] = {static_cast<cuuint64_t>(head_dim), rows, 2 * static_cast<cuuint64_t>(v.num_blocks)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim), rows * head_dim};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(head_dim), kUnit, 1}, steps[3] = {1, 1, 1};
+    const CUtensorMapSwizzle swizzle = head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, v.codes, sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+template <int D, bool INT8, int NT, bool SCORES>
 cudaError_t launch(const BlockAttentionParams& p, cudaStream_t stream) {
-    using C = Config<D, INT8, NT>;
+    using C = Config<D, INT8, NT, SCORES>;
     static std::atomic<uint64_t> prepared{0};  // devices whose shared-memory limit was raised
     int device = 0;
     cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return err;
-    if (C::kSmem > 48 * 1024 && (device >= 64 || !(prepared.load(std::memory_order_relaxed) >> device & 1))) {
+    if ((device >= 64 || !(prepared.load(std::memory_order_relaxed) >> device & 1))) {
         err = cudaFuncSetAttribute(block_attention_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        if (err == cudaSuccess) err = cudaFuncSetAttribute(block_attention_kernel<C>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         if (err != cudaSuccess) return err;
         if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     const bool programmatic = p.programmatic_launch != 0;
-    err = launch_chained(block_attention_kernel<C>, p, dim3(static_cast<unsigned>(p.spans)), kThreads, C::kSmem, 1, programmatic, stream);
+    AttentionLaunch launch;
+    launch.p = p;
+    if ((err = describe_codes(p.v, D, &launch.map)) != cudaSuccess) return err;
+    err = launch_chained(block_attention_kernel<C>, launch, dim3(static_cast<unsigned>(p.spans)), kThreads, C::kSmem, 1, programmatic, stream);
     if (err == cudaSuccess && p.max_len > kChunk)  // items of one chunk are never cut
-        err = launch_chained(block_join_kernel<C>, p, dim3(static_cast<unsigned>(p.num_rows) * p.heads), kThreads, 0, 1, programmatic, stream);
-    if (err == cudaSuccess && p.accumulate) {
-        const unsigned parts = static_cast<unsigned>(std::min(64, (p.max_len + kThreads - 1) / kThreads));
+        err = launch_chained(block_join_kernel<Config<D, INT8, NT, false>>, p, dim3(static_cast<unsigned>(p.join_ctas), static_cast<unsigned>(p.join_parts)), kJoinWarps * 32, 0, 1, programmatic, stream);
+    if (err == cudaSuccess && SCORES) {
+        const unsigned parts = static_cast<unsigned>(std::min(64, (p.max_len + 4 * kThreads - 1) / (4 * kThreads)));
         if (parts > 0)
             err = launch_chained(block_weights_kernel, p, dim3(static_cast<unsigned>(p.v.num_requests) * p.v.kv_heads, parts), kThreads, 0, 1,
                                  programmatic, stream);
@@ -678,13 +855,20 @@ cudaError_t launch(const BlockAttentionParams& p, cudaStream_t stream) {
 
 template <int D, bool INT8>
 cudaError_t launch_tiles(const BlockAttentionParams& p, cudaStream_t stream) {
-    return p.query_tiles == 1 ? launch<D, INT8, 1>(p, stream) : launch<D, INT8, 2>(p, stream);
+    if (p.query_tiles == 1) return p.accumulate ? launch<D, INT8, 1, true>(p, stream) : launch<D, INT8, 1, false>(p, stream);
+    return p.accumulate ? launch<D, INT8, 2, true>(p, stream) : launch<D, INT8, 2, false>(p, stream);
 }
 
 }  // namespace
 
 int block_attention_slot_floats(int head_dim, int query_tiles) { return 8 * query_tiles * (head_dim + 4); }
-int block_attention_chunk() { return kChunk; }
+cudaError_t block_attention_status(cudaStream_t stream, int* status) {
+    const cudaError_t err = cudaMemcpyFromSymbolAsync(status, g_block_attention_status, sizeof(*status), 0, cudaMemcpyDeviceToHost, stream);
+    return err == cudaSuccess ? cudaStreamSynchronize(stream) : err;
+}
+
+int64_t block_attention_units(int tokens) { return std::max(1, (tokens + kChunk - 1) / kChunk) + kItemCost; }
+int block_attention_resident(int query_tiles) { return resident(query_tiles); }
 
 cudaError_t launch_block_attention(const BlockAttentionParams& p, int head_dim, int int8, cudaStream_t stream) {
     if (head_dim == 128) return int8 ? launch_tiles<128, true>(p, stream) : launch_tiles<128, false>(p, stream);

@@ -638,9 +638,9 @@ static int block_view(const RqBlockCache& c, const RqBlockBatch& b, bool rows, r
     if (c.element != RQ_BLOCK_E4M3 && c.element != RQ_BLOCK_INT8)
         return fail(RQ_ERR_UNSUPPORTED, "unknown block-cache element %d", c.element);
     if (c.kv_heads < 1 || c.num_blocks < 1) return fail(RQ_ERR_INVALID_ARGUMENT, "a block cache needs at least one head and one block");
-    if (c.kv_heads > 65535 || c.num_blocks > 0x7fffffff) return fail(RQ_ERR_INVALID_ARGUMENT, "too many heads or blocks in one cache");
-    if (c.codes == nullptr || !aligned(c.codes, 16) || c.scales == nullptr || !aligned(c.scales, 4) || !aligned(c.weights, 4))
-        return fail(RQ_ERR_INVALID_ARGUMENT, "16-byte aligned 8-bit codes [2, blocks, heads, page tokens, channels] and fp32 scales required");
+    if (c.kv_heads > 65535 || c.num_blocks > 0x3fffffff) return fail(RQ_ERR_INVALID_ARGUMENT, "too many heads or blocks in one cache");
+    if (c.codes == nullptr || !aligned(c.codes, 16) || c.scales == nullptr || !aligned(c.scales, 4) || !aligned(c.weights, 16))
+        return fail(RQ_ERR_INVALID_ARGUMENT, "16-byte aligned 8-bit codes [2, blocks, heads, page tokens, channels], fp32 scales and 16-byte aligned weights required");
     if (b.num_requests < 1 || b.seq_lens == nullptr || (b.block_table == nullptr && b.max_blocks_per_request > 0) || (rows && b.query_start_loc == nullptr))
         return fail(RQ_ERR_INVALID_ARGUMENT, "int32 query starts [requests+1], sequence lengths [requests] and page table required");
     if (b.max_blocks_per_request < 0 || b.block_table_stride < b.max_blocks_per_request || b.max_blocks_per_request > 0x7fffffff / 32)
@@ -732,23 +732,31 @@ static int block_attention_params(const RqBlockAttentionArgs* a, rq::BlockAttent
     // evenly over the requests; any spread is right).
     const int64_t rows_each = (static_cast<int64_t>(a->num_rows) + a->batch.num_requests - 1) / a->batch.num_requests;
     p->query_tiles = rows_each * p->group <= 8 ? 1 : 2;
-    // One span for each resident CTA, fewer where the batch cannot have that many chunks.
-    const int64_t per_item = (static_cast<int64_t>(p->max_len) + rq::block_attention_chunk() - 1) / rq::block_attention_chunk();
+    // One span for each resident CTA, fewer where the batch cannot have that many units of work.
     const int64_t items = (static_cast<int64_t>(a->num_rows) * p->group / (8 * p->query_tiles) + a->batch.num_requests) * a->cache.kv_heads;
-    const int64_t resident = (p->query_tiles == 1 ? 4LL : 3LL) * current_sm_count();
+    const int64_t units = items * rq::block_attention_units(p->max_len), resident = static_cast<int64_t>(rq::block_attention_resident(p->query_tiles)) * current_sm_count();
     p->min_span = 1;
-    p->spans = static_cast<int>(per_item == 0 || per_item * items > resident ? resident : per_item * items);
+    p->spans = static_cast<int>(units > resident ? resident : units);
     // workspace: unfinished pieces, then what an accumulating call leaves for its last launch
     const size_t partials = round_up(static_cast<size_t>(2) * p->spans * rq::block_attention_slot_floats(a->cache.head_dim, p->query_tiles) * sizeof(float), 256);
+    const size_t cuts = round_up(static_cast<size_t>(p->spans) * sizeof(rq::BlockCut), 256);
     const size_t lse = p->accumulate ? round_up(static_cast<size_t>(a->num_rows) * a->heads * sizeof(float), 256) : 0;
     p->score_stride = (static_cast<int64_t>(p->max_len) + 7) / 8 * 8;
     const size_t scores = p->accumulate ? round_up(static_cast<size_t>(a->num_rows) * a->heads * p->score_stride * sizeof(float), 256) : 0;
-    *workspace = partials + lse + scores;
-    p->partials = static_cast<float*>(a->workspace);
-    if (p->accumulate && a->workspace != nullptr) {
-        p->row_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + partials);
-        p->scores = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + partials + lse);
+    *workspace = partials + cuts + lse + scores;
+    uint8_t* base = static_cast<uint8_t*>(a->workspace);
+    if (base != nullptr) {
+        p->partials = reinterpret_cast<float*>(base);
+        p->cuts = reinterpret_cast<rq::BlockCut*>(base + partials);
+        if (p->accumulate) {
+            p->row_lse = reinterpret_cast<float*>(base + partials + cuts);
+            p->scores = reinterpret_cast<float*>(base + partials + cuts + lse);
+        }
     }
+    // Where there are few items each can have many pieces: every query is joined by a CTA of its own, and fewer CTAs look for
+    // the items, neighbouring spans each (items of many pieces begin far apart).
+    p->join_parts = items * 8 <= current_sm_count() ? 8 : 2;
+    p->join_ctas = p->join_parts == 8 && p->spans > current_sm_count() ? current_sm_count() : p->spans;
     return RQ_OK;
 }
 
@@ -773,6 +781,13 @@ int32_t rq_block_attention(const RqBlockAttentionArgs* a) {
     return err == cudaSuccess ? RQ_OK : fail_cuda(err, "block attention launch");
 }
 
+int32_t rq_block_attention_status(void* stream) {
+    int status = 0;
+    const cudaError_t err = rq::block_attention_status(static_cast<cudaStream_t>(stream), &status);
+    if (err != cudaSuccess) return fail_cuda(err, "block attention status");
+    return status == 0 ? RQ_OK : fail(RQ_ERR_DEVICE_TIMEOUT, "a bounded wait inside the block attention kernel gave up");
+}
+
 int32_t rq_block_evict(const RqBlockEvictArgs* a) {
     if (a == nullptr) return fail(RQ_ERR_INVALID_ARGUMENT, "null arguments");
     rq::BlockEvictParams p;
@@ -793,9 +808,14 @@ int32_t rq_block_evict(const RqBlockEvictArgs* a) {
     p.recent = a->recent;
     p.kept = a->kept;
     p.new_lens = a->new_lens;
-    // CTAs per (request, KV head): up to eight while that keeps the grid within one wave of two CTAs per multiprocessor
+    // CTAs per (request, KV head): as many (up to eight) as keep the grid within two per multiprocessor and leave each at least
+    // 1024 of the tokens that a request can have; small CTAs where there are enough pairs to fill the GPU four deep.
+    const int64_t most = static_cast<int64_t>(p.v.max_blocks) * p.v.page_tokens;
     p.cluster = 1;
-    while (p.cluster < 8 && pairs * p.cluster * 2 <= 2LL * current_sm_count()) p.cluster *= 2;
+    while (p.cluster < 8 && pairs * p.cluster <= current_sm_count() && most / (2 * p.cluster) >= 1024) p.cluster *= 2;
+    p.threads = pairs * p.cluster > 2LL * current_sm_count() ? 256 : 512;
+    const int64_t share = (most + p.cluster - 1) / p.cluster + 8;  // of the candidates, from a multiple of four on
+    p.key_room = static_cast<int>(share < rq::kBlockEvictKeys ? (share + 3) / 4 * 4 : rq::kBlockEvictKeys);
     p.programmatic_launch = chained(a->flags);
     const cudaError_t err = rq::launch_block_evict(p, a->cache.head_dim, a->cache.element == RQ_BLOCK_INT8, static_cast<cudaStream_t>(a->stream));
     return err == cudaSuccess ? RQ_OK : fail_cuda(err, "block evict launch");

@@ -146,6 +146,13 @@ struct BlockAppendParams {
 };
 cudaError_t launch_block_append(const BlockAppendParams& p, int head_dim, int int8, cudaStream_t stream);
 
+// An item of attention work that goes on behind the span that it begins in.
+struct BlockCut {
+    int pieces;   // spans that take part, 0: there is no such item
+    int inside;   // its first piece is not the span's first
+    int first, queries, query0, head;  // first row of its request, queries from query0 on, its first query, KV head
+};
+
 struct BlockAttentionParams {
     BlockView v;
     const void* query;
@@ -156,23 +163,29 @@ struct BlockAttentionParams {
     float scale_log2;        // softmax scale * log2(e)
     float* lse;              // or nullptr
     int query_tiles;         // eights of queries that a CTA takes together
-    int spans, min_span;     // CTAs that the work is cut for, and the fewest chunks each takes
+    int spans, min_span;     // CTAs that the work is cut for, and the fewest units each takes
     float* partials;         // workspace [2 * spans][8 * query_tiles][head_dim + 4]: value sums, m, l, M of unfinished pieces
+    BlockCut* cuts;          // workspace [spans]
+    int join_ctas, join_parts;  // of the join: CTAs that share out the spans, CTAs for each of them
     float* scores;           // workspace [num_rows][heads][score_stride]: scores times log2(e) (accumulate), or nullptr
     float* row_lse;          // workspace [num_rows][heads]: log2 of the softmax denominators (accumulate), or nullptr
     int64_t score_stride;
     int programmatic_launch;
 };
-int block_attention_chunk();  // tokens that spans are counted in
+int64_t block_attention_units(int tokens);  // of work that an item of this many tokens is counted as
+int block_attention_resident(int query_tiles);  // CTAs on a multiprocessor
 int block_attention_slot_floats(int head_dim, int query_tiles);
+cudaError_t block_attention_status(cudaStream_t stream, int* status);  // of the current device; synchronizes
 cudaError_t launch_block_attention(const BlockAttentionParams& p, int head_dim, int int8, cudaStream_t stream);
 
+constexpr int kBlockEvictKeys = 16384;  // most weights a CTA keeps in shared memory
 struct BlockEvictParams {
     BlockView v;
     int budget, sinks, recent;
     int32_t* kept;
     int32_t* new_lens;       // or nullptr
-    int cluster;             // CTAs per (request, KV head)
+    int cluster, threads;    // CTAs per (request, KV head), threads of each (256 or 512)
+    int key_room;            // weights that a CTA keeps in shared memory (a multiple of 4)
     int programmatic_launch;
 };
 cudaError_t launch_block_evict(const BlockEvictParams& p, int head_dim, int int8, cudaStream_t stream);

@@ -73,7 +73,7 @@ def check_attention(cache, batch, query, *, scale=None, accumulate=False, pad=0,
     out = torch.full_like(query, 77.0)
     lse = torch.full(query.shape[:2], 55.0, device=DEVICE)
     cache.attention(query, out, *batch.meta, softmax_scale=scale, lse=lse, accumulate=accumulate, **more)
-    torch.cuda.synchronize()
+    cache.attention_status()
     want, want_lse, magnitude, spread, added = oracle.attention(query, batch.starts, batch.lengths, batch.table, scale, accumulate,
                                                                 more.get("max_seq_len"))
     real = batch.starts[-1]
