@@ -277,15 +277,15 @@ def load() -> ctypes.CDLL:
     lib.rq_peer_open.restype = ctypes.c_int32
     lib.rq_peer_close.argtypes = [ctypes.c_void_p]
     lib.rq_peer_close.restype = ctypes.c_int32
-    lib.rq_block_append.argtypes = [ctypes.POINTER(RqBlockAppendArgs)]
+    lib.rq_block_append.argtypes = [ctypes.c_void_p]   # RqBlockAppendArgs, or its bytes
     lib.rq_block_append.restype = ctypes.c_int32
-    lib.rq_block_attention.argtypes = [ctypes.POINTER(RqBlockAttentionArgs)]
+    lib.rq_block_attention.argtypes = [ctypes.c_void_p]   # RqBlockAttentionArgs, or its bytes
     lib.rq_block_attention.restype = ctypes.c_int32
-    lib.rq_block_attention_workspace_bytes.argtypes = [ctypes.POINTER(RqBlockAttentionArgs)]
+    lib.rq_block_attention_workspace_bytes.argtypes = [ctypes.c_void_p]
     lib.rq_block_attention_workspace_bytes.restype = ctypes.c_size_t
     lib.rq_block_attention_status.argtypes = [ctypes.c_void_p]
     lib.rq_block_attention_status.restype = ctypes.c_int32
-    lib.rq_block_evict.argtypes = [ctypes.POINTER(RqBlockEvictArgs)]
+    lib.rq_block_evict.argtypes = [ctypes.c_void_p]   # RqBlockEvictArgs, or its bytes
     lib.rq_block_evict.restype = ctypes.c_int32
     lib.rq_last_error.argtypes = []
     lib.rq_last_error.restype = ctypes.c_char_p

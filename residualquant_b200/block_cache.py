@@ -23,7 +23,7 @@ raise RuntimeError.
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -35,6 +35,13 @@ __all__ = ("BlockCache",)
 
 _ELEMENTS = {torch.float8_e4m3fn: 0, torch.int8: 1}
 _ACTIVATIONS = {torch.bfloat16: 0, torch.float16: 1}
+
+# A decode step issues these calls once for each layer, so the argument structures of include/rq_b200.h are packed in one go
+# (a tenth of what filling them field by field takes).
+_CACHE, _BATCH = "PPPqiiii", "PPPiii4x"
+_APPEND = struct.Struct("@" + _CACHE + _BATCH + "PPqqiiPi4x")
+_ATTENTION = struct.Struct("@" + _CACHE + _BATCH + "PPqqiiiif4xPi4xPNPi4x")
+_EVICT = struct.Struct("@" + _CACHE + _BATCH + "iii4xPPPi4x")
 
 
 class BlockCache:
@@ -66,8 +73,9 @@ class BlockCache:
         self.num_blocks, self.kv_heads, self.block_size, self.head_dim = blocks, heads, block_size, head_dim
         self.device = codes.device
         self._lib = _lib.load()
-        self._view = _lib.RqBlockCache(codes.data_ptr(), scales.data_ptr(), weights.data_ptr() if weights is not None else None,
-                                       blocks, heads, head_dim, block_size, _ELEMENTS[codes.dtype])
+        self._view = (codes.data_ptr(), scales.data_ptr(), weights.data_ptr() if weights is not None else 0,
+                      blocks, heads, head_dim, block_size, _ELEMENTS[codes.dtype])
+        self._workspaces = {}   # bytes that an attention call of some sizes needs
 
     @classmethod
     def allocate(cls, num_blocks: int, kv_heads: int, head_dim: int, block_size: int = 16, dtype: torch.dtype = torch.float8_e4m3fn,
@@ -77,43 +85,43 @@ class BlockCache:
         scales = torch.ones(2, num_blocks, kv_heads, device=device)
         return cls(codes, scales, torch.zeros(num_blocks, kv_heads, block_size, device=device) if weights else None)
 
-    def _batch(self, query_start_loc, seq_lens, block_table) -> _lib.RqBlockBatch:
-        device, requests = self.device, seq_lens.numel()
-        _require(
-            seq_lens.device == device and seq_lens.dtype == torch.int32 and seq_lens.dim() == 1 and seq_lens.is_contiguous(),
-            "Contiguous INT32 sequence lengths required",
-        )
-        _require(
-            query_start_loc is None
-            or (query_start_loc.device == device and query_start_loc.dtype == torch.int32 and query_start_loc.dim() == 1
-                and query_start_loc.is_contiguous() and query_start_loc.numel() == requests + 1),
-            "Contiguous INT32 query starts with one final boundary required",
-        )
-        _require(
-            block_table.device == device and block_table.dtype == torch.int32 and block_table.dim() == 2
-            and (block_table.stride(1) == 1 or block_table.size(1) <= 1) and block_table.size(0) >= requests
-            and block_table.stride(0) >= block_table.size(1),
-            "INT32 page table with packed rows required",
-        )
-        return _lib.RqBlockBatch(query_start_loc.data_ptr() if query_start_loc is not None else None, seq_lens.data_ptr(),
-                                 block_table.data_ptr(), requests, block_table.stride(0), block_table.size(1))
+    def _batch(self, query_start_loc, seq_lens, block_table) -> tuple:
+        device = self.device
+        if not (seq_lens.device == device and seq_lens.dtype == torch.int32 and seq_lens.dim() == 1 and seq_lens.is_contiguous()):
+            raise RuntimeError("Contiguous INT32 sequence lengths required")
+        requests = seq_lens.numel()
+        starts = 0
+        if query_start_loc is not None:
+            if not (query_start_loc.device == device and query_start_loc.dtype == torch.int32 and query_start_loc.dim() == 1
+                    and query_start_loc.is_contiguous() and query_start_loc.numel() == requests + 1):
+                raise RuntimeError("Contiguous INT32 query starts with one final boundary required")
+            starts = query_start_loc.data_ptr()
+        if not (block_table.device == device and block_table.dtype == torch.int32 and block_table.dim() == 2):
+            raise RuntimeError("INT32 page table with packed rows required")
+        rows, width = block_table.shape
+        row_stride, stride = block_table.stride()
+        if not ((stride == 1 or width <= 1) and rows >= requests and (row_stride >= width or rows <= 1)):
+            raise RuntimeError("INT32 page table with packed rows required")
+        return starts, seq_lens.data_ptr(), block_table.data_ptr(), requests, max(row_stride, width), width
 
-    def _rows(self, t: torch.Tensor, heads: int, what: str) -> None:
-        _require(
-            t.device == self.device and t.dtype in _ACTIVATIONS and t.dim() == 3 and t.size(1) == heads and t.size(2) == self.head_dim
-            and t.stride(2) == 1 and (heads == 1 or t.stride(1) == self.head_dim),
-            f"BF16 or FP16 [tokens, {heads}, {self.head_dim}] {what} with packed trailing strides on the cache device required",
-        )
+    def _rows(self, t: torch.Tensor, heads: int, what: str) -> int:
+        """The stride between the rows of [rows, heads, head dim]."""
+        if t.device == self.device and t.dtype in _ACTIVATIONS and t.dim() == 3:
+            _, own_heads, dim = t.shape
+            stride, head_stride, unit = t.stride()
+            if own_heads == heads and dim == self.head_dim and unit == 1 and (heads == 1 or head_stride == dim):
+                return stride
+        raise RuntimeError(f"BF16 or FP16 [tokens, {heads}, {self.head_dim}] {what} with packed trailing strides on the cache device required")
 
-    def _call(self, function, args) -> None:
-        index = self.device.index
-        if torch.cuda.current_device() == index:
-            args.stream = torch.cuda.current_stream(index).cuda_stream
-            status = function(ctypes.byref(args))
+    def _stream(self) -> int:
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def _call(self, function, args: bytes) -> None:
+        if torch.cuda.current_device() == self.device.index:
+            status = function(args)
         else:
-            with torch.cuda.device(index):
-                args.stream = torch.cuda.current_stream(index).cuda_stream
-                status = function(ctypes.byref(args))
+            with torch.cuda.device(self.device.index):
+                status = function(args)
         if status != _lib.RQ_OK:
             _lib.check(status)
 
@@ -124,15 +132,16 @@ class BlockCache:
         A block that the call begins (its slot 0 is written) takes the scale of its new tokens; a block that held earlier
         tokens of the request keeps its scale or, where the new tokens need a larger one, takes that and has the earlier
         tokens rounded again.  The new tokens' accumulated weights start at 0."""
-        for t, what in ((key, "key"), (value, "value")):
-            self._rows(t, self.kv_heads, what)
-        _require(key.dtype == value.dtype and key.size(0) == value.size(0), "K and V must match in type and row count")
+        key_stride, value_stride = self._rows(key, self.kv_heads, "key"), self._rows(value, self.kv_heads, "value")
+        rows = key.size(0)
+        if key.dtype != value.dtype or value.size(0) != rows:
+            raise RuntimeError("K and V must match in type and row count")
         batch = self._batch(query_start_loc, seq_lens, block_table)
-        if key.size(0) == 0 or seq_lens.numel() == 0:
-            return
-        args = _lib.RqBlockAppendArgs(self._view, batch, key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0),
-                                      key.size(0), _ACTIVATIONS[key.dtype])
-        self._call(self._lib.rq_block_append, args)
+        if rows and batch[3]:
+            row = self.kv_heads * self.head_dim
+            self._call(self._lib.rq_block_append, _APPEND.pack(
+                *self._view, *batch, key.data_ptr(), value.data_ptr(), key_stride if rows > 1 else row, value_stride if rows > 1 else row,
+                rows, _ACTIVATIONS[key.dtype], self._stream(), 0))
 
     def attention(self, query: torch.Tensor, output: torch.Tensor, query_start_loc: torch.Tensor, seq_lens: torch.Tensor,
                   block_table: torch.Tensor, *, softmax_scale: Optional[float] = None, lse: Optional[torch.Tensor] = None,
@@ -143,34 +152,45 @@ class BlockCache:
         `softmax_scale` defaults to head_dim ** -0.5.  Rows that see no token get zeros and -inf; padding rows stay as they are.
 
         `accumulate` adds every token's softmax weight, summed over the rows and over the query heads of its KV head, to the
-        cache's `weights`.  Such a call needs scratch memory for rows x heads x `max_seq_len` scores; `max_seq_len` (default: the
-        block table's width) must be no smaller than any of `seq_lens`: tokens behind it are not seen."""
+        cache's `weights`.  Such a call needs scratch memory for rows x heads x `max_seq_len` scores.  `max_seq_len` (default: the
+        block table's width) must be no smaller than any of `seq_lens`: tokens behind it are not seen; up to 256 saves a launch."""
         heads = query.size(1) if query.dim() == 3 else 0
-        self._rows(query, heads, "query")
-        self._rows(output, heads, "output")
-        _require(output.dtype == query.dtype and output.size(0) == query.size(0), "Q and output must match in type and row count")
-        _require(heads > 0 and heads % self.kv_heads == 0, f"{heads} query heads are no multiple of the cache's {self.kv_heads} heads")
-        for t in (query, output):
-            _require(t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0, "Q/output addresses and token strides must be 16-byte aligned")
-        _require(
-            lse is None
-            or (lse.device == self.device and lse.dtype == torch.float32 and lse.is_contiguous()
-                and tuple(lse.shape) == (query.size(0), heads)),
-            "Contiguous FP32 [tokens, heads] lse required",
-        )
-        _require(not accumulate or self.weights is not None, "accumulating needs a cache with weights")
-        _require(max_seq_len is None or max_seq_len > 0, "max_seq_len must be positive")
+        query_stride, output_stride = self._rows(query, heads, "query"), self._rows(output, heads, "output")
+        rows = query.size(0)
+        if output.dtype != query.dtype or output.size(0) != rows:
+            raise RuntimeError("Q and output must match in type and row count")
+        if heads == 0 or heads % self.kv_heads:
+            raise RuntimeError(f"{heads} query heads are no multiple of the cache's {self.kv_heads} heads")
+        if rows <= 1:
+            query_stride = output_stride = heads * self.head_dim
+        query_address, output_address = query.data_ptr(), output.data_ptr()
+        if (query_address | output_address) % 16 or (query_stride | output_stride) % 8:
+            raise RuntimeError("Q/output addresses and token strides must be 16-byte aligned")
+        if lse is not None and not (lse.device == self.device and lse.dtype == torch.float32 and lse.is_contiguous()
+                                    and lse.shape == (rows, heads)):
+            raise RuntimeError("Contiguous FP32 [tokens, heads] lse required")
+        if accumulate and self.weights is None:
+            raise RuntimeError("accumulating needs a cache with weights")
+        if max_seq_len is not None and max_seq_len <= 0:
+            raise RuntimeError("max_seq_len must be positive")
         batch = self._batch(query_start_loc, seq_lens, block_table)
-        if query.size(0) == 0 or seq_lens.numel() == 0:
+        if not rows or not batch[3]:
             return
-        args = _lib.RqBlockAttentionArgs(
-            self._view, batch, query.data_ptr(), output.data_ptr(), query.stride(0), output.stride(0), query.size(0), heads,
-            _ACTIVATIONS[query.dtype], bool(accumulate), self.head_dim ** -0.5 if softmax_scale is None else softmax_scale,
-            lse.data_ptr() if lse is not None else None, min(max_seq_len or 0, 0x7FFFFFFF))
-        nbytes = self._lib.rq_block_attention_workspace_bytes(ctypes.byref(args))
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
-        self._call(self._lib.rq_block_attention, args)
+        scale = self.head_dim ** -0.5 if softmax_scale is None else softmax_scale
+        if not 0.0 < scale < 1e30:
+            raise RuntimeError("softmax scale must be positive and finite")
+        front = (*self._view, *batch, query_address, output_address, query_stride, output_stride, rows, heads, _ACTIVATIONS[query.dtype],
+                 bool(accumulate), scale, lse.data_ptr() if lse is not None else 0, min(max_seq_len or 0, 0x7FFFFFFF))
+        sizes = (rows, heads, batch[3], batch[5], bool(accumulate), max_seq_len)
+        nbytes = self._workspaces.get(sizes)
+        if nbytes is None:
+            nbytes = self._lib.rq_block_attention_workspace_bytes(_ATTENTION.pack(*front, 0, 0, 0, 0))
+            if len(self._workspaces) >= 4096:
+                self._workspaces.clear()
+            self._workspaces[sizes] = nbytes
+        workspace = self.codes.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        self._call(self._lib.rq_block_attention,
+                   _ATTENTION.pack(*front, workspace.data_ptr() if nbytes else 0, nbytes, self._stream(), 0))
 
     def attention_status(self) -> None:
         """Synchronize and raise if a bounded wait inside an attention kernel of any block cache ever gave up on this device."""
@@ -186,28 +206,25 @@ class BlockCache:
 
         Returns `kept` int32 [requests, kv heads, budget], the positions that the tokens now at 0, 1, ... had before (-1 behind
         the last), and `new_lens` int32 [requests], min(seq_len, budget); both can be passed in (not `seq_lens` itself)."""
-        _require(self.weights is not None, "evicting needs a cache with weights")
-        _require(budget >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget,
-                 f"A budget of {budget} tokens cannot hold the first {sinks} and the last {recent}")
+        if self.weights is None:
+            raise RuntimeError("evicting needs a cache with weights")
+        if not (1 <= budget < 1 << 24 and sinks >= 0 and recent >= 0 and sinks + recent <= budget):
+            raise RuntimeError(f"A budget of {budget} tokens cannot hold the first {sinks} and the last {recent}")
         batch = self._batch(None, seq_lens, block_table)
-        requests = seq_lens.numel()
+        requests = batch[3]
         if kept is None:
             kept = torch.empty(requests, self.kv_heads, budget, dtype=torch.int32, device=self.device)
+        elif not (kept.device == self.device and kept.dtype == torch.int32 and kept.is_contiguous()
+                  and kept.shape == (requests, self.kv_heads, budget)):
+            raise RuntimeError("Contiguous INT32 [requests, heads, budget] kept positions required")
         if new_lens is None:
             new_lens = torch.empty(requests, dtype=torch.int32, device=self.device)
-        _require(
-            kept.device == self.device and kept.dtype == torch.int32 and kept.is_contiguous()
-            and tuple(kept.shape) == (requests, self.kv_heads, budget),
-            "Contiguous INT32 [requests, heads, budget] kept positions required",
-        )
-        _require(
-            new_lens.device == self.device and new_lens.dtype == torch.int32 and new_lens.is_contiguous()
-            and tuple(new_lens.shape) == (requests,),
-            "Contiguous INT32 [requests] new lengths required",
-        )
-        _require(abs(new_lens.data_ptr() - seq_lens.data_ptr()) >= 4 * requests or requests == 0,
-                 "new_lens must not share memory with seq_lens")
+        elif not (new_lens.device == self.device and new_lens.dtype == torch.int32 and new_lens.is_contiguous()
+                  and new_lens.shape == (requests,)):
+            raise RuntimeError("Contiguous INT32 [requests] new lengths required")
         if requests:
-            self._call(self._lib.rq_block_evict,
-                       _lib.RqBlockEvictArgs(self._view, batch, budget, sinks, recent, kept.data_ptr(), new_lens.data_ptr()))
+            if abs(new_lens.data_ptr() - batch[1]) < 4 * requests:
+                raise RuntimeError("new_lens must not share memory with seq_lens")
+            self._call(self._lib.rq_block_evict, _EVICT.pack(
+                *self._view, *batch, budget, sinks, recent, kept.data_ptr(), new_lens.data_ptr(), self._stream(), 0))
         return kept, new_lens

@@ -5,9 +5,10 @@
 //   code = rne(x / s); where s grew, the earlier tokens' codes become rne(code * s_old / s)
 //
 // One warp owns a (block, KV head, plane) for the whole call: it is the only reader and writer of that scale, so the result
-// depends on no order and needs no atomics.  The warp that does the work is the one at the block's first new row (a "leader"
-// row: the request's first row, or one whose position starts a block); the tokens stay in registers between the maximum and
-// the encoding, so every row is read once.  Memory bound: 2 bytes read and 1 written per element.
+// depends on no order and needs no atomics.  The warp that does the work is the one at the block's first new row (the
+// request's first row, or one whose position starts a block); the tokens stay in registers between the maximum and the
+// encoding, so every row is read once.  Finding the request, position and page costs three dependent loads, so a warp goes on
+// to other heads and planes of the block where there are warps enough.  Memory bound: 2 bytes read and 1 written per element.
 #include "rq_block_common.cuh"
 
 namespace rq {
@@ -15,36 +16,56 @@ namespace {
 
 constexpr int kAppendWarps = 8;
 
+// Eight activations -> eight codes, for finite values that the scale brings into range.
 template <bool INT8>
-__device__ __forceinline__ uint2 encode8(const uint4& x, float inverse, bool fp16) {
+__device__ __forceinline__ uint2 encode8_finite(const uint4& x, float inverse, bool fp16) {
+    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+    uint32_t pairs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = activation2(words[i], fp16);
+        if constexpr (INT8) {
+            // x / scale + 1.5 * 2^23 rounds to a whole number (ties to even), whose low byte is the code
+            const float magic = 12582912.f;
+            pairs[i] = __byte_perm(__float_as_uint(fmaf(f.x, inverse, magic)), __float_as_uint(fmaf(f.y, inverse, magic)), 0x0040);
+        } else {
+            pairs[i] = __nv_cvt_float2_to_fp8x2(make_float2(f.x * inverse, f.y * inverse), __NV_SATFINITE, __NV_E4M3);
+        }
+    }
+    return make_uint2(__byte_perm(pairs[0], pairs[1], 0x5410), __byte_perm(pairs[2], pairs[3], 0x5410));
+}
+
+// The same with infinities and NaN among them.
+template <bool INT8>
+__device__ __noinline__ uint2 encode8(uint4 x, float inverse, bool fp16) {
     const float2 a = activation2(x.x, fp16), b = activation2(x.y, fp16), c = activation2(x.z, fp16), d = activation2(x.w, fp16);
     return make_uint2(encode2<INT8>(a.x * inverse, a.y * inverse) | (encode2<INT8>(b.x * inverse, b.y * inverse) << 16),
                       encode2<INT8>(c.x * inverse, c.y * inverse) | (encode2<INT8>(d.x * inverse, d.y * inverse) << 16));
 }
 
-__device__ __forceinline__ uint32_t finite_magnitude(float x) {
-    const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
-    return bits < 0x7f800000u ? bits : 0u;
+// Largest of two pairs' 16-bit magnitudes, pair by pair.
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b & 0x7fff7fffu); }
+// 16-bit magnitude bits, of finite values only.
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t pair, uint32_t infinity) {
+    const uint32_t low = pair & 0x7fffu, high = (pair >> 16) & 0x7fffu;
+    return max(low < infinity ? low : 0u, high < infinity ? high : 0u);
 }
 
 template <int D, int P, bool INT8>
 __global__ void __launch_bounds__(kAppendWarps * 32) block_append_kernel(const BlockAppendParams p) {
     constexpr int kRow = D / 8;             // pieces of eight channels in a row
-    constexpr int kPieces = P * kRow / 32;  // pieces a lane holds
+    constexpr int kPieces = P * kRow / 32;  // pieces of a block that a lane holds
     const BlockView& v = p.v;
     const int lane = threadIdx.x & 31;
-    const int planes = 2 * v.kv_heads;
+    const int strips = 2 * v.kv_heads, groups = (strips + p.strips - 1) / p.strips;  // a strip: one head of one plane
     const int64_t warp = static_cast<int64_t>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
-    const int64_t piece_of_rows = warp / planes;
+    const int64_t chunk = warp / groups;
     pdl_wait();
     pdl_launch_dependents();
-    if (piece_of_rows * p.chunk >= p.num_rows) return;
-    const int head = static_cast<int>(warp % planes) >> 1, plane = static_cast<int>(warp % planes) & 1;
-    int row = static_cast<int>(piece_of_rows) * p.chunk;
+    if (chunk * p.chunk >= p.num_rows) return;
+    const int first_strip = static_cast<int>(warp % groups) * p.strips, last_strip = min(strips, first_strip + p.strips);
+    int row = static_cast<int>(chunk) * p.chunk;
     const int end = min(row + p.chunk, p.num_rows);
-    const int64_t page_bytes = static_cast<int64_t>(P) * D;
-    const int64_t stride = p.stride[plane];
-    const uint16_t* source = static_cast<const uint16_t*>(p.rows[plane]);
 
     int r = find_request(v.query_start_loc, v.num_requests, row, lane);
     while (row < end && r < v.num_requests) {
@@ -55,17 +76,21 @@ __global__ void __launch_bounds__(kAppendWarps * 32) block_append_kernel(const B
         if (position < 0) { row += min(-position, last - row); continue; }  // rows before the sequence's start hold no token
         const int old = position % P;  // slots of the block that are taken already
         if (old != 0 && row != first) { row += min(P - old, last - row); continue; }
-        const int count = min(P - old, last - row);
+        const int count = min(P - old, last - row), block_row = row;
+        row += count;
         const int64_t id = block_id(v, r, position / P);
-        if (id >= 0) {
+        if (id < 0) continue;
+        for (int strip = first_strip; strip < last_strip; ++strip) {
+            const int plane = strip >= v.kv_heads ? 1 : 0, head = strip - plane * v.kv_heads;
+            const int64_t stride = p.stride[plane];
+            const uint16_t* source = static_cast<const uint16_t*>(p.rows[plane]) + block_row * stride + head * D;
             uint4 x[kPieces];
-            uint32_t amax = 0u;
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 const int piece = i * 32 + lane, token = piece / kRow - old, channel = (piece % kRow) * 8;
                 x[i] = make_uint4(0u, 0u, 0u, 0u);
                 if (token >= 0 && token < count) {
-                    const uint16_t* at = source + (row + token) * stride + head * D + channel;
+                    const uint16_t* at = source + token * stride + channel;
                     if (p.vector_loads) {
                         x[i] = *reinterpret_cast<const uint4*>(at);
                     } else {
@@ -73,22 +98,28 @@ __global__ void __launch_bounds__(kAppendWarps * 32) block_append_kernel(const B
                     }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const uint32_t words[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = activation2(words[j], p.fp16);
-                    amax = max(amax, max(finite_magnitude(f.x), finite_magnitude(f.y)));
-                }
-            }
-            amax = __reduce_max_sync(kFullMask, amax);
-            float* scale_at = v.scales + (static_cast<int64_t>(plane) * v.num_blocks + id) * v.kv_heads + head;
-            uint8_t* page = v.codes + ((static_cast<int64_t>(plane) * v.num_blocks + id) * v.kv_heads + head) * page_bytes;
+            const int64_t page_index = (plane * v.num_blocks + id) * v.kv_heads + head;
+            float* scale_at = v.scales + page_index;
+            uint8_t* page = v.codes + page_index * (P * D);
             float before = old != 0 ? *scale_at : 0.f;
             if (!(before > 0.f && before < INFINITY)) before = 0.f;
-            float scale = amax != 0u ? block_scale<INT8>(amax) : 0.f;
-            scale = fmaxf(scale, before);
+            // the largest magnitude, on the 16-bit patterns: they are ordered like the values
+            const uint32_t infinity = p.fp16 ? 0x7c00u : 0x7f80u;
+            uint32_t largest = 0u;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) largest = larger(larger(larger(larger(largest, x[i].x), x[i].y), x[i].z), x[i].w);
+            uint32_t bits = __reduce_max_sync(kFullMask, max(largest & 0xffffu, largest >> 16));
+            const bool finite = bits < infinity;
+            if (!finite) {
+                bits = 0u;
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i)
+                    bits = max(bits, max(max(finite_or_zero(x[i].x, infinity), finite_or_zero(x[i].y, infinity)),
+                                         max(finite_or_zero(x[i].z, infinity), finite_or_zero(x[i].w, infinity))));
+                bits = __reduce_max_sync(kFullMask, bits);
+            }
+            const uint32_t amax = __float_as_uint(activation2(bits, p.fp16).x);
+            float scale = fmaxf(amax != 0u ? block_scale<INT8>(amax) : 0.f, before);
             if (scale == 0.f) scale = 1.f;
             if (old != 0 && scale > before) {
                 const float ratio = before / scale;
@@ -108,20 +139,19 @@ __global__ void __launch_bounds__(kAppendWarps * 32) block_append_kernel(const B
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 const int piece = i * 32 + lane, token = piece / kRow - old;
-                if (token >= 0 && token < count) *reinterpret_cast<uint2*>(page + piece * 8) = encode8<INT8>(x[i], inverse, p.fp16);
+                if (token >= 0 && token < count)
+                    *reinterpret_cast<uint2*>(page + piece * 8) = finite ? encode8_finite<INT8>(x[i], inverse, p.fp16) : encode8<INT8>(x[i], inverse, p.fp16);
             }
-            __syncwarp();
+            __syncwarp();  // every lane has read the scale
             if (lane == 0) *scale_at = scale;
-            if (plane == 0 && v.weights != nullptr && lane < count)
-                v.weights[(id * v.kv_heads + head) * P + old + lane] = 0.f;
+            if (plane == 0 && v.weights != nullptr && lane < count) v.weights[(id * v.kv_heads + head) * P + old + lane] = 0.f;
         }
-        row += count;
     }
 }
 
 template <int D, int P>
 cudaError_t launch_append(const BlockAppendParams& p, int int8, cudaStream_t stream) {
-    const int64_t warps = (static_cast<int64_t>(p.num_rows) + p.chunk - 1) / p.chunk * 2 * p.v.kv_heads;
+    const int64_t warps = (static_cast<int64_t>(p.num_rows) + p.chunk - 1) / p.chunk * ((2 * p.v.kv_heads + p.strips - 1) / p.strips);
     const dim3 grid(static_cast<unsigned>((warps + kAppendWarps - 1) / kAppendWarps));
     const bool programmatic = p.programmatic_launch != 0;
     return int8 ? launch_chained(block_append_kernel<D, P, true>, p, grid, kAppendWarps * 32, 0, 1, programmatic, stream)

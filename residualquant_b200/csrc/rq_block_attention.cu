@@ -17,11 +17,12 @@
 // from losing either.
 //
 // Memory bound: 2 D bytes for each cached token and KV head.  All items' tokens, in chunks of kChunk and kItemCost chunks
-// more for each item, are laid end to end and cut into equal spans, one for each CTA (four per SM, three with sixteen queries, all resident), whatever
-// the lengths are; the spans are found on the device from the lengths, so that a captured launch stays right.  A span that
-// ends inside an item leaves (m, l, M, O) in the workspace, and a second launch joins those.  Each warp streams its own
-// 16-token units through a ring of cp.async stages, and the next item's first units are set off before the warps join the
-// results of this one.
+// more for each item, are laid end to end and cut into equal spans, one for each CTA (four per SM, three with sixteen queries;
+// all resident), whatever the lengths are; the spans are found on the device from the lengths, so that a captured launch
+// stays right.  A span that ends inside an item leaves (m, l, M, O) in the workspace, and a second launch joins those.
+// Each warp streams its own 16-token units: one lane has the tensor-memory engine copy a unit's rows of K and V into a ring of
+// shared-memory stages.  (Copies by all threads, cp.async, kept the load/store unit busy: 40 sequences x 2200 tokens x 8
+// heads took 58 us instead of 46.)  The next item's first units are set off before the warps join the results of this one.
 #include <cuda.h>
 
 #include <algorithm>
@@ -118,23 +119,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-// Four cached bytes -> two fp16 pairs (bytes 0, 1 and bytes 2, 3), exact.  int8: a byte with its sign bit flipped is
-// u = code + 128; the fp16 pattern 0x6400 | u is 1024 + u.
-template <bool INT8>
-__device__ __forceinline__ void to_half(uint32_t word, uint32_t& low, uint32_t& high) {
-    if constexpr (INT8) {
-        const uint32_t u = word ^ 0x80808080u;
-        const __half2 bias = __float2half2_rn(1152.f);
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
-        low = *reinterpret_cast<const uint32_t*>(&x);
-        high = *reinterpret_cast<const uint32_t*>(&y);
-    } else {
-        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-            : "=r"(low), "=r"(high) : "r"(word));
-    }
-}
-
 // Where 16-byte piece `piece` of token `token` stands in a plane of a stage.  128-byte rows have their pieces rotated by xor
 // with the token (the copy's 128-byte swizzle), so that the reads of eight rows (K) and of eight pieces of every second row (V)
 // meet no bank twice; 64-byte rows the same by pairs (K's reads meet none, V's two); 96-byte rows are packed, and K's 8-byte
@@ -151,6 +135,7 @@ struct Request {
     int first, queries, tokens;  // first row, rows * group, tokens that its last row sees at most
     int before;                  // tokens ahead of its first row (may be negative)
     int tiles, chunks;
+    int cost;                    // units of work that an item counts: its chunks and a fixed part, or 1 where items are not cut
 };
 template <int ROWS>
 __device__ __forceinline__ Request request_from(const BlockAttentionParams& p, int first, int last, int length) {
@@ -161,6 +146,7 @@ __device__ __forceinline__ Request request_from(const BlockAttentionParams& p, i
     q.before = length - (last - first);
     q.tiles = (q.queries + ROWS - 1) / ROWS;
     q.chunks = max(1, (q.tokens + kChunk - 1) / kChunk);
+    q.cost = p.whole_items ? 1 : q.chunks + kItemCost;
     return q;
 }
 template <int ROWS>
@@ -168,7 +154,7 @@ __device__ __forceinline__ Request request_of(const BlockAttentionParams& p, int
     return request_from<ROWS>(p, p.v.query_start_loc[r], p.v.query_start_loc[r + 1], p.v.seq_lens[r]);
 }
 __device__ __forceinline__ int64_t work_of(const BlockAttentionParams& p, const Request& q) {
-    return static_cast<int64_t>(q.tiles) * p.v.kv_heads * (q.chunks + kItemCost);
+    return static_cast<int64_t>(q.tiles) * p.v.kv_heads * q.cost;
 }
 
 // Where things stand in the list of all items: each takes kItemCost units and one for each chunk, and the list is cut into
@@ -255,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
     pdl_launch_dependents();
     const Place start = find_place<kRows, kWarps>(p, place_shared, blockIdx.x);
     const int64_t begin = blockIdx.x * start.span, end = min(begin + start.span, start.total);
-    if (tid == 0) p.cuts[blockIdx.x].pieces = 0;  // until an item is found that goes on in the next span
+    if (tid == 0 && !p.whole_items) p.cuts[blockIdx.x].pieces = 0;  // until an item is found that goes on in the next span
     if (begin >= end) return;
     const int64_t plane_scales = v.num_blocks * v.kv_heads;
     uint8_t* ring = smem + warp * kStages * C::kStage;
@@ -296,10 +282,10 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
                 q = request_of<kRows>(p, ++r);
                 continue;
             }
-            const int cost = q.chunks + kItemCost;
+            const int cost = q.cost;
             const int item = static_cast<int>(local / cost), done = static_cast<int>(local - static_cast<int64_t>(item) * cost);
             const int upto = static_cast<int>(min(static_cast<int64_t>(cost), done + (end - at)));
-            const int chunk0 = max(0, done - kItemCost), chunk1 = upto - kItemCost;
+            const int chunk0 = p.whole_items ? 0 : max(0, done - kItemCost), chunk1 = p.whole_items ? q.chunks : upto - kItemCost;
             // a span leaves at most two unfinished pieces: one that goes on at its start, and one that begins inside it
             slot = 2LL * blockIdx.x + (at == begin && done >= kItemCost ? 0 : 1);
             at += upto - done;
@@ -842,7 +828,7 @@ cudaError_t launch(const BlockAttentionParams& p, cudaStream_t stream) {
     launch.p = p;
     if ((err = describe_codes(p.v, D, &launch.map)) != cudaSuccess) return err;
     err = launch_chained(block_attention_kernel<C>, launch, dim3(static_cast<unsigned>(p.spans)), kThreads, C::kSmem, 1, programmatic, stream);
-    if (err == cudaSuccess && p.max_len > kChunk)  // items of one chunk are never cut
+    if (err == cudaSuccess && !p.whole_items)
         err = launch_chained(block_join_kernel<Config<D, INT8, NT, false>>, p, dim3(static_cast<unsigned>(p.join_ctas), static_cast<unsigned>(p.join_parts)), kJoinWarps * 32, 0, 1, programmatic, stream);
     if (err == cudaSuccess && SCORES) {
         const unsigned parts = static_cast<unsigned>(std::min(64, (p.max_len + 4 * kThreads - 1) / (4 * kThreads)));
@@ -867,7 +853,9 @@ cudaError_t block_attention_status(cudaStream_t stream, int* status) {
     return err == cudaSuccess ? cudaStreamSynchronize(stream) : err;
 }
 
-int64_t block_attention_units(int tokens) { return std::max(1, (tokens + kChunk - 1) / kChunk) + kItemCost; }
+// Items of up to four chunks are not cut: a CTA takes about as long for them as for the join of two halves.
+bool block_attention_whole(int tokens) { return tokens <= 4 * kChunk; }
+int64_t block_attention_units(int tokens) { return block_attention_whole(tokens) ? 1 : (tokens + kChunk - 1) / kChunk + kItemCost; }
 int block_attention_resident(int query_tiles) { return resident(query_tiles); }
 
 cudaError_t launch_block_attention(const BlockAttentionParams& p, int head_dim, int int8, cudaStream_t stream) {

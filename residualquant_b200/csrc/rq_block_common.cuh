@@ -41,6 +41,23 @@ __device__ __forceinline__ uint32_t encode2(float a, float b) {
     }
 }
 
+// Four cached bytes -> two fp16 pairs (bytes 0, 1 and bytes 2, 3), exact.  int8: a byte with its sign bit flipped is
+// u = code + 128; the fp16 pattern 0x6400 | u is 1024 + u.
+template <bool INT8>
+__device__ __forceinline__ void to_half(uint32_t word, uint32_t& low, uint32_t& high) {
+    if constexpr (INT8) {
+        const uint32_t u = word ^ 0x80808080u;
+        const __half2 bias = __float2half2_rn(1152.f);
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+        low = *reinterpret_cast<const uint32_t*>(&x);
+        high = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(low), "=r"(high) : "r"(word));
+    }
+}
+
 // A 16-bit activation pair -> two floats.
 __device__ __forceinline__ float2 activation2(uint32_t pair, bool fp16) {
     if (fp16) {
@@ -62,9 +79,9 @@ __device__ __forceinline__ uint32_t pack_activation2(float a, float b, bool fp16
 }
 
 // Request that row `row` belongs to: the last r with starts[r] <= row, num_requests for a padding row.  One warp searches
-// 32 boundaries at a time; a batch of single-token requests, where row r is request r, is recognised first.
+// 32 boundaries at a time; a large batch of single-token requests, where row r is request r, is recognised first.
 __device__ __forceinline__ int find_request(const int32_t* starts, int num_requests, int row, int lane) {
-    if (row < num_requests && starts[row] <= row && row < starts[row + 1]) return row;
+    if (num_requests >= 32 && row < num_requests && starts[row] <= row && row < starts[row + 1]) return row;
     int lo = 0, hi = num_requests + 1;
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32, i = lo + lane * step;

@@ -7,11 +7,12 @@
 // passes give the key of the last kept candidate and how many candidates equal to it are kept (the first ones); each warp then
 // lists the kept tokens of its stretch behind those of the stretches before it.
 // Compaction: kept token i moves to position i, and no kept token stands before its new position, so the destination
-// blocks are done in ascending waves, a (block, plane) to a warp: a wave reads all its sources into registers, the cluster meets,
-// then the wave is written.  Later waves read only blocks behind everything written so far.
+// blocks are done in ascending waves, a (block, plane) to a warp: a wave reads all its sources into shared memory, the cluster
+// meets, then the wave is written.  Later waves read only blocks behind everything written so far, so they can be read ahead.
 // Memory bound: weights once, kept tokens once each way.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "rq_block_common.cuh"
@@ -32,6 +33,31 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+// Whether codes times `ratio` are exact in fp16, down to e4m3's and int8's smallest steps: a power of two of moderate size.
+__device__ __forceinline__ bool moves_exactly(float ratio) {
+    return (__float_as_uint(ratio) & 0x007fffffu) == 0u && ratio >= 6.103515625e-05f && ratio <= 128.f;
+}
+
+// Four codes times `ratio`, rounded to codes again; exact products in fp16, one rounding.
+template <bool INT8>
+__device__ __forceinline__ uint32_t move_codes(uint32_t word, __half2 ratio) {
+    uint32_t low, high;
+    to_half<INT8>(word, low, high);
+    __half2 a = *reinterpret_cast<__half2*>(&low), b = *reinterpret_cast<__half2*>(&high);
+    if constexpr (INT8) {
+        // + 1536 rounds to a whole number (ties to even), whose low byte is the code
+        const __half2 magic = __float2half2_rn(1536.f);
+        a = __hfma2(a, ratio, magic);
+        b = __hfma2(b, ratio, magic);
+        return __byte_perm(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b), 0x6420);
+    } else {
+        a = __hmul2(a, ratio);
+        b = __hmul2(b, ratio);
+        return static_cast<uint32_t>(__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(a), __NV_SATFINITE, __NV_E4M3)) |
+               (static_cast<uint32_t>(__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(b), __NV_SATFINITE, __NV_E4M3)) << 16);
+    }
+}
+
 struct EvictShared {
     uint32_t histogram[kBins];
     uint32_t greater[kMaxWarps], equal[kMaxWarps];  // a warp's candidates above / at the threshold
@@ -40,7 +66,7 @@ struct EvictShared {
 };
 
 template <int D, int P, bool INT8>
-__global__ void __launch_bounds__(kMaxWarps * 32, 2) block_evict_kernel(const BlockEvictParams p) {
+__global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_kernel(const BlockEvictParams p) {
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ EvictShared shared;
     const cg::cluster_group cluster = cg::this_cluster();
@@ -197,86 +223,120 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) block_evict_kernel(const Bl
         if (i < p.sinks) kept[i] = i;
         else kept[p.budget - p.recent + i - p.sinks] = n - p.recent + i - p.sinks;
     }
-    meet();  // the list is complete and visible to the cluster; no CTA's shared memory is read from here on
+    meet();  // the list is complete and visible to the cluster; the keys and other CTAs' shared memory are done with
 
     // ---- compaction ----
+    // A warp's item of a wave goes through three steps, each a wave ahead of the next: where its tokens are (lane i: token i),
+    // their codes into shared memory, and the move.
     constexpr int kRow = D / 16;               // 16-byte pieces of a token
-    constexpr int kPieces = P * kRow / 32;     // pieces of a block that a lane holds
+    constexpr int kPieces = P * kRow / 32;     // pieces of a block that a lane moves
+    uint4* staged = reinterpret_cast<uint4*>(keys) + warp * 2 * P * kRow;
     const int items = 2 * ((p.budget + P - 1) / P), wave = size * warps;
-    int item = rank * warps + warp;
-    int count;              // kept tokens of the item's block
-    int64_t source;         // lane i: page that its token comes from (-1: none), slot there, scale and weight
-    int slot;
-    float scale, moved;
-    auto look_up = [&]() {
-        const int first = (item >> 1) * P;
-        count = item < items ? min(P, p.budget - first) : 0;
-        source = -1;
-        slot = 0;
-        scale = moved = 0.f;
-        if (lane < count) {
-            const int token = __ldcg(kept + first + lane);
-            const int id = table[token / P];
-            slot = token % P;
-            if (valid(id)) {
-                const int64_t page = static_cast<int64_t>(id) * v.kv_heads + head;
-                source = (item & 1) * v.num_blocks * v.kv_heads + page;
-                scale = __ldcg(v.scales + source);
-                if ((item & 1) == 0) moved = __ldcg(v.weights + page * P + slot);
-            }
+    struct Place {
+        int count;            // kept tokens of the block
+        int id, slot;         // lane i: page that token i comes from (-1: none) and its slot there
+        int to;               // page that the block goes to
+        float scale, moved;   // lane i: scale and weight of token i
+    };
+    auto count_of = [&](int item) { return item < items ? min(P, p.budget - (item >> 1) * P) : 0; };
+    auto token_of = [&](int item) { return lane < count_of(item) ? __ldcg(kept + (item >> 1) * P + lane) : 0; };
+    auto find = [&](Place& at, int item, int token) {
+        at.count = count_of(item);
+        at.id = lane < at.count ? table[token / P] : -1;
+        at.slot = token % P;
+        at.to = at.count > 0 ? table[item >> 1] : -1;
+    };
+    auto load_scales = [&](Place& at, int item) {
+        if (!valid(at.id)) at.id = -1;
+        at.scale = at.moved = 0.f;
+        if (at.id >= 0) {
+            const int64_t page = static_cast<int64_t>(at.id) * v.kv_heads + head;
+            at.scale = __ldcg(v.scales + (item & 1) * v.num_blocks * v.kv_heads + page);
+            if ((item & 1) == 0) at.moved = __ldcg(v.weights + page * P + at.slot);
         }
     };
-    look_up();
-    for (int done = 0; done < items; done += wave) {
-        uint4 code[kPieces];
+    auto load_codes = [&](const Place& at, int item, int stage) {
+        const uint8_t* plane = v.codes + (item & 1) * v.num_blocks * v.kv_heads * P * D;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int piece = i * 32 + lane, token = piece / kRow;
-            const int64_t from_page = __shfl_sync(kFullMask, source, token);
-            const int from_slot = __shfl_sync(kFullMask, slot, token);
-            code[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (from_page >= 0) code[i] = __ldcg(reinterpret_cast<const uint4*>(v.codes + (from_page * P + from_slot) * D + (piece % kRow) * 16));
+            const int id = __shfl_sync(kFullMask, at.id, token), slot = __shfl_sync(kFullMask, at.slot, token);
+            const uint8_t* from = plane + (((id >= 0 ? id : 0) * static_cast<int64_t>(v.kv_heads) + head) * P + slot) * D + (piece % kRow) * 16;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(staged + stage * P * kRow + piece))),
+                         "l"(from), "r"(id >= 0 ? 16 : 0) : "memory");
         }
-        const int now_count = count, now_item = item;
-        const float now_scale = scale, now_moved = moved;
-        item += wave;
-        look_up();  // the next wave's sources, while this one's codes are on their way
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int item = rank * warps + warp, stage = 0;
+    Place now, then;
+    find(now, item, token_of(item));
+    int token = token_of(item + wave);
+    load_scales(now, item);
+    load_codes(now, item, 0);
+    find(then, item + wave, token);
+    token = token_of(item + 2 * wave);
+    load_scales(then, item + wave);
+    for (int done = 0; done < items; done += wave) {
+        Place later;
+        load_codes(then, item + wave, stage ^ 1);
+        find(later, item + 2 * wave, token);
+        token = token_of(item + 3 * wave);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
         uint32_t amax = 0u;
+        const uint4* codes = staged + stage * P * kRow + lane;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const uint32_t words[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
-            float largest = 0.f;
+            const uint4 code = codes[i * 32];
+            const uint32_t words[4] = {code.x, code.y, code.z, code.w};
+            __half2 largest = __float2half2_rn(0.f);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 a = decode2<INT8>(words[j]), b = decode2<INT8>(words[j] >> 16);
-                largest = fmaxf(largest, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
+                uint32_t low, high;
+                to_half<INT8>(words[j], low, high);
+                largest = __hmax2(largest, __hmax2(__habs2(*reinterpret_cast<__half2*>(&low)), __habs2(*reinterpret_cast<__half2*>(&high))));
             }
-            const uint32_t bits = __float_as_uint(largest * __shfl_sync(kFullMask, now_scale, (i * 32 + lane) / kRow));
+            const float2 both = __half22float2(largest);
+            const uint32_t bits = __float_as_uint(fmaxf(both.x, both.y) * __shfl_sync(kFullMask, now.scale, (i * 32 + lane) / kRow));
             if (bits < 0x7f800000u) amax = max(amax, bits);
         }
         amax = __reduce_max_sync(kFullMask, amax);
         const float fresh = amax != 0u ? block_scale<INT8>(amax) : 1.f;
-        const float inverse = 1.f / fresh;
-        meet();  // every source of this wave is in registers
-        const int to_id = now_count > 0 ? table[now_item >> 1] : -1;
-        const bool write = valid(to_id);
-        const int64_t page = static_cast<int64_t>(to_id) * v.kv_heads + head, plane_page = (now_item & 1) * v.num_blocks * v.kv_heads + page;
+        const float own_ratio = now.scale * (1.f / fresh);
+        const bool exact = __all_sync(kFullMask, lane >= now.count || moves_exactly(own_ratio));
+        meet();  // every source of this wave has been read
+        const bool write = valid(now.to);
+        const int64_t page = static_cast<int64_t>(now.to) * v.kv_heads + head, plane_page = (item & 1) * v.num_blocks * v.kv_heads + page;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int piece = i * 32 + lane;
-            const float ratio = __shfl_sync(kFullMask, now_scale, piece / kRow) * inverse;
-            if (!write || piece / kRow >= now_count) continue;
-            uint32_t words[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+            const float ratio = __shfl_sync(kFullMask, own_ratio, piece / kRow);
+            const uint4 code = codes[i * 32];
+            uint32_t words[4] = {code.x, code.y, code.z, code.w};
+            if (exact) {
+                const __half2 half_ratio = __float2half2_rn(ratio);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 a = decode2<INT8>(words[j]), b = decode2<INT8>(words[j] >> 16);
-                words[j] = encode2<INT8>(a.x * ratio, a.y * ratio) | (encode2<INT8>(b.x * ratio, b.y * ratio) << 16);
+                for (int j = 0; j < 4; ++j) words[j] = move_codes<INT8>(words[j], half_ratio);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 a = decode2<INT8>(words[j]), b = decode2<INT8>(words[j] >> 16);
+                    words[j] = encode2<INT8>(a.x * ratio, a.y * ratio) | (encode2<INT8>(b.x * ratio, b.y * ratio) << 16);
+                }
             }
-            *reinterpret_cast<uint4*>(v.codes + plane_page * P * D + piece * 16) = make_uint4(words[0], words[1], words[2], words[3]);
+            if (write && piece / kRow < now.count)
+                *reinterpret_cast<uint4*>(v.codes + plane_page * P * D + piece * 16) = make_uint4(words[0], words[1], words[2], words[3]);
         }
         if (write && lane == 0) v.scales[plane_page] = fresh;
-        if (write && (now_item & 1) == 0 && lane < now_count) v.weights[page * P + lane] = now_moved;
+        if (write && (item & 1) == 0 && lane < now.count) v.weights[page * P + lane] = now.moved;
+        load_scales(later, item + 2 * wave);
+        now = then;
+        then = later;
+        item += wave;
+        stage ^= 1;
+        __syncwarp();
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <int D, int P, bool INT8>
@@ -287,12 +347,13 @@ cudaError_t launch_evict(const BlockEvictParams& p, cudaStream_t stream) {
     cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return err;
     if (device >= 64 || !(prepared.load(std::memory_order_relaxed) >> device & 1)) {
-        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockEvictKeys * 4);
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(kBlockEvictKeys * 4, kMaxWarps * 2 * P * D));
         if (err != cudaSuccess) return err;
         if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     const dim3 grid(static_cast<unsigned>(p.v.num_requests) * p.v.kv_heads * p.cluster);
-    return launch_chained(kernel, p, grid, p.threads, static_cast<size_t>(p.key_room) * 4, p.cluster, p.programmatic_launch != 0, stream);
+    const size_t staged = static_cast<size_t>(p.threads / 32) * 2 * P * D;
+    return launch_chained(kernel, p, grid, p.threads, std::max(static_cast<size_t>(p.key_room) * 4, staged), p.cluster, p.programmatic_launch != 0, stream);
 }
 
 template <int D>

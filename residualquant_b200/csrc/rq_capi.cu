@@ -683,12 +683,15 @@ int32_t rq_block_append(const RqBlockAppendArgs* a) {
     p.num_rows = a->num_rows;
     p.fp16 = a->activation == RQ_ACTIVATION_FP16;
     p.vector_loads = aligned(a->key, 16) && aligned(a->value, 16) && a->key_stride % 8 == 0 && a->value_stride % 8 == 0;
-    // Rows a warp walks over in search of the blocks that begin there: one while that leaves enough warps to fill the GPU
-    // (single-token steps), up to a block's worth for prompts, where only every page_tokens-th row begins a block.
-    p.chunk = 1;
-    while (p.chunk < a->cache.page_tokens &&
-           static_cast<int64_t>(a->num_rows) * 2 * a->cache.kv_heads / (2 * p.chunk) >= 16LL * current_sm_count())
-        p.chunk *= 2;
+    // Rows a warp walks over in search of the blocks that begin there: up to a block's worth, but not more than requests have
+    // on average (single-token steps begin a block in every row).  Then heads and planes that it takes.  Both while 24 warps
+    // are left for each multiprocessor: 41,521 prompt rows x 16 heads take 119 us with one head and plane to a warp, 96 with
+    // four, 102 with eight.
+    p.chunk = p.strips = 1;
+    int64_t warps = static_cast<int64_t>(a->num_rows) * 2 * a->cache.kv_heads;
+    const int64_t enough = 24LL * current_sm_count(), rows_each = a->num_rows / a->batch.num_requests;
+    for (; 2 * p.chunk <= rows_each && p.chunk < a->cache.page_tokens && warps / 2 >= enough; warps /= 2) p.chunk *= 2;
+    for (; p.strips < 4 && warps / 2 >= enough; warps /= 2) p.strips *= 2;
     if ((static_cast<int64_t>(a->num_rows) + p.chunk - 1) / p.chunk * 2 * a->cache.kv_heads / 8 >= 0x7fffffffLL)
         return fail(RQ_ERR_INVALID_ARGUMENT, "too many rows in one call");
     p.programmatic_launch = chained(a->flags);
@@ -736,10 +739,11 @@ static int block_attention_params(const RqBlockAttentionArgs* a, rq::BlockAttent
     const int64_t items = (static_cast<int64_t>(a->num_rows) * p->group / (8 * p->query_tiles) + a->batch.num_requests) * a->cache.kv_heads;
     const int64_t units = items * rq::block_attention_units(p->max_len), resident = static_cast<int64_t>(rq::block_attention_resident(p->query_tiles)) * current_sm_count();
     p->min_span = 1;
+    p->whole_items = rq::block_attention_whole(p->max_len) ? 1 : 0;
     p->spans = static_cast<int>(units > resident ? resident : units);
     // workspace: unfinished pieces, then what an accumulating call leaves for its last launch
-    const size_t partials = round_up(static_cast<size_t>(2) * p->spans * rq::block_attention_slot_floats(a->cache.head_dim, p->query_tiles) * sizeof(float), 256);
-    const size_t cuts = round_up(static_cast<size_t>(p->spans) * sizeof(rq::BlockCut), 256);
+    const size_t partials = p->whole_items ? 0 : round_up(static_cast<size_t>(2) * p->spans * rq::block_attention_slot_floats(a->cache.head_dim, p->query_tiles) * sizeof(float), 256);
+    const size_t cuts = p->whole_items ? 0 : round_up(static_cast<size_t>(p->spans) * sizeof(rq::BlockCut), 256);
     const size_t lse = p->accumulate ? round_up(static_cast<size_t>(a->num_rows) * a->heads * sizeof(float), 256) : 0;
     p->score_stride = (static_cast<int64_t>(p->max_len) + 7) / 8 * 8;
     const size_t scores = p->accumulate ? round_up(static_cast<size_t>(a->num_rows) * a->heads * p->score_stride * sizeof(float), 256) : 0;
@@ -774,7 +778,7 @@ int32_t rq_block_attention(const RqBlockAttentionArgs* a) {
     const int status = block_attention_params(a, &p, &need);
     if (status != RQ_OK) return status;
     if (a->num_rows == 0) return RQ_OK;
-    if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < need)
+    if (need != 0 && (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < need))
         return fail(RQ_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu", need, a->workspace_bytes);
     p.programmatic_launch = chained(a->flags);
     const cudaError_t err = rq::launch_block_attention(p, a->cache.head_dim, a->cache.element == RQ_BLOCK_INT8, static_cast<cudaStream_t>(a->stream));

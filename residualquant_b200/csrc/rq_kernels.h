@@ -141,7 +141,7 @@ struct BlockAppendParams {
     int num_rows;
     int fp16;                // activations are fp16 (else bf16)
     int vector_loads;        // rows are 16-byte aligned
-    int chunk;               // rows that one warp walks over
+    int chunk, strips;       // rows that one warp walks over, and heads of a plane (K's, then V's) that it takes
     int programmatic_launch;
 };
 cudaError_t launch_block_append(const BlockAppendParams& p, int head_dim, int int8, cudaStream_t stream);
@@ -164,6 +164,7 @@ struct BlockAttentionParams {
     float* lse;              // or nullptr
     int query_tiles;         // eights of queries that a CTA takes together
     int spans, min_span;     // CTAs that the work is cut for, and the fewest units each takes
+    int whole_items;         // items are not cut: no join
     float* partials;         // workspace [2 * spans][8 * query_tiles][head_dim + 4]: value sums, m, l, M of unfinished pieces
     BlockCut* cuts;          // workspace [spans]
     int join_ctas, join_parts;  // of the join: CTAs that share out the spans, CTAs for each of them
@@ -173,6 +174,7 @@ struct BlockAttentionParams {
     int programmatic_launch;
 };
 int64_t block_attention_units(int tokens);  // of work that an item of this many tokens is counted as
+bool block_attention_whole(int tokens);     // whether items of up to this many tokens are not cut
 int block_attention_resident(int query_tiles);  // CTAs on a multiprocessor
 int block_attention_slot_floats(int head_dim, int query_tiles);
 cudaError_t block_attention_status(cudaStream_t stream, int* status);  // of the current device; synchronizes

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from residualquant_b200 import _lib
+from residualquant_b200 import _lib, block_cache
 from residualquant_b200.block_cache import BlockCache
 
 ADDRESS = 1 << 20   # a pointer that is only looked at
@@ -73,7 +73,8 @@ def test_attention_refuses(built_library, changes):
 
 def test_attention_asks_for_its_workspace(built_library):
     lib = _lib.load()
-    args = attention_args()
+    wide = dict(block_table_stride=100, max_blocks_per_request=100)
+    args = attention_args(**wide)
     need = lib.rq_block_attention_workspace_bytes(ctypes.byref(args))
     assert need > 0 and need % 256 == 0
     assert lib.rq_block_attention(ctypes.byref(args)) == -3                 # none given
@@ -82,9 +83,12 @@ def test_attention_asks_for_its_workspace(built_library):
     args.workspace, args.workspace_bytes = ADDRESS + 16, need
     assert lib.rq_block_attention(ctypes.byref(args)) == -3
     assert lib.rq_block_attention(ctypes.byref(attention_args(num_rows=0))) == 0
-    # the scores of an accumulating call: rows x heads x the length bound
-    counted = lib.rq_block_attention_workspace_bytes(ctypes.byref(attention_args(accumulate=1)))
-    assert counted >= need
+    # the scores and denominators of an accumulating call: rows x heads x the length bound
+    counted = lib.rq_block_attention_workspace_bytes(ctypes.byref(attention_args(accumulate=1, **wide)))
+    assert counted == need + 256 + 3 * 8 * 1600 * 4
+    # short tables: no item is cut, so only what is accumulated
+    assert lib.rq_block_attention_workspace_bytes(ctypes.byref(attention_args())) == 0
+    assert lib.rq_block_attention_workspace_bytes(ctypes.byref(attention_args(accumulate=1))) == 256 + 3 * 8 * 64 * 4
 
 
 @pytest.mark.parametrize("changes", BAD_CACHE + [dict(weights=None), dict(), dict(budget=4, sinks=3, recent=2), dict(budget=4, sinks=-1),
@@ -96,6 +100,21 @@ def test_evict_refuses(built_library, changes):
         changes = dict(budget=4, **changes)
     assert lib.rq_block_evict(ctypes.byref(evict_args(**changes))) < 0
     assert lib.rq_block_evict(None) == -1
+
+
+def test_packed_arguments_have_the_layout_of_the_structures():
+    for packed, kind in ((block_cache._APPEND, _lib.RqBlockAppendArgs), (block_cache._ATTENTION, _lib.RqBlockAttentionArgs),
+                         (block_cache._EVICT, _lib.RqBlockEvictArgs)):
+        assert packed.size == ctypes.sizeof(kind)
+        flat = []
+        for name, field in kind._fields_:
+            inner = getattr(field, "_fields_", None)
+            flat += [(name, n) for n, _ in inner] if inner else [(name,)]
+        values = packed.pack(*range(1, len(flat) + 1))          # a whole number for every field, the float among them
+        args = kind.from_buffer_copy(values)
+        for i, path in enumerate(flat):
+            field = getattr(args, path[0])
+            assert (getattr(field, path[1]) if len(path) == 2 else field) == i + 1, path
 
 
 def test_the_cache_lives_on_the_gpu(built_library):
