@@ -69,7 +69,10 @@ struct Config {
     static constexpr int kOffInfo = kWarps * kStages * kStage;        // float4 [warps][stages]: K scale, log2 of V's, tokens
     static constexpr int kOffStat = kOffInfo + kWarps * kStages * 16; // float [warps][8][4]: m, l, M, the stage of the sums
     static constexpr int kOffQuery = kOffStat + kWarps * 8 * 16;      // 16-bit [rows][D]: the next piece's queries
-    static constexpr int kOffBarrier = kOffQuery + kRows * D * 2;     // uint64 [warps][stages]
+    // sixteen queries would take too many registers: their fp16 fragments stay in shared memory, [n][pair of steps][lane]
+    static constexpr bool kSharedQueries = NT > 1;
+    static constexpr int kOffFragments = kOffQuery + kRows * D * 2;
+    static constexpr int kOffBarrier = kOffFragments + (kSharedQueries ? kRows * D * 2 : 0);  // uint64 [warps][stages]
     static constexpr int kOffPlace = kOffBarrier + kWarps * kStages * 8;
     static constexpr int kSmem = kOffPlace + 64;
     static constexpr int kSlot = D + 4;                               // floats a query's partial result takes
@@ -366,7 +369,8 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 
     while (more) {
         // the queries as fp16
-        uint32_t qf[NT][kSteps][2];
+        uint32_t qf[C::kSharedQueries ? 1 : NT][kSteps][2];
+        uint4* const fragments = reinterpret_cast<uint4*>(smem + C::kOffFragments) + lane;
         float factor[NT][2];   // score units of queries 8 n + 2 t + {0, 1}
         int limit[NT][2];      // tokens that they see
         int least = 0x7fffffff;
@@ -401,8 +405,13 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 f = activation2(raw[s][i], p.fp16);
-                    qf[n][s][i] = pack_activation2(f.x * down, f.y * down, true);
+                    qf[C::kSharedQueries ? 0 : n][s][i] = pack_activation2(f.x * down, f.y * down, true);
                 }
+            }
+            if constexpr (C::kSharedQueries) {  // every warp has all of them, and writes its share
+#pragma unroll
+                for (int s = 0; s < kSteps; s += 2)
+                    if ((n * kSteps + s) / 2 % kWarps == warp) fragments[(n * kSteps + s) / 2 * 32] = make_uint4(qf[0][s][0], qf[0][s][1], qf[0][s + 1][0], qf[0][s + 1][1]);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -413,6 +422,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
             }
         }
         least = __reduce_min_sync(kFullMask, least);
+        if constexpr (C::kSharedQueries) __syncthreads();
         float* score_at[NT][2];
         if constexpr (C::kScores) {
 #pragma unroll
@@ -488,12 +498,23 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
                 }
             }
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                uint32_t a[4];
+            for (int s = 0; s < kSteps; s += 2) {
+                uint32_t a[4], b[4];
                 to_half<C::kInt8>(low[s], a[0], a[2]);
                 to_half<C::kInt8>(high[s], a[1], a[3]);
+                to_half<C::kInt8>(low[s + 1], b[0], b[2]);
+                to_half<C::kInt8>(high[s + 1], b[1], b[3]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma(s & 1 ? x_odd[n] : x[n], a, qf[n][s][0], qf[n][s][1]);
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (C::kSharedQueries) {
+                        const uint4 f = fragments[(n * kSteps + s) / 2 * 32];
+                        mma(x[n], a, f.x, f.y);
+                        mma(x_odd[n], b, f.z, f.w);
+                    } else {
+                        mma(x[n], a, qf[n][s][0], qf[n][s][1]);
+                        mma(x_odd[n], b, qf[n][s + 1][0], qf[n][s + 1][1]);
+                    }
+                }
             }
             const float value_scale = about.y;
             const bool masked = count < kUnit || token0 + kUnit > least;

@@ -62,6 +62,7 @@ struct EvictShared {
     uint32_t histogram[kBins];
     uint32_t greater[kMaxWarps], equal[kMaxWarps];  // a warp's candidates above / at the threshold
     uint32_t digit, above;                          // digit found by a pass, candidates above it
+    uint32_t slice;                                 // candidates of all CTAs in this CTA's slice of the bins
     uint32_t all_greater, all_equal;                // this CTA's
 };
 
@@ -139,16 +140,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
                 const uint32_t key = key_of(token);
                 if (pass == 0 || (key >> (kShift[pass] & 31)) == prefix) atomicAdd(&shared.histogram[(key >> shift) & (bins - 1)], 1u);
             }
+            // Bins from the top down: the digit is where the count reaches `missing`.  Each CTA of a cluster adds up a slice of all
+            // CTAs' bins (slice 0 the topmost), and the one whose slice the count is reached in finds the digit.
+            const int width = bins / size, mine_from = bins - (rank + 1) * width;
             meet();
-            // bins from the top down, eight for each of the first 256 threads: the digit is where the count reaches `missing`
             uint32_t mine[8], sum = 0u;
-            const int high = bins - 1 - tid * 8;
+            const int high = mine_from + width - 1 - tid * 8;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mine[j] = high - j >= 0 ? shared.histogram[high - j] : 0u;
-            if (size > 1) {
+            for (int j = 0; j < 8; ++j) mine[j] = 0u;
+            if (size == 1) {
 #pragma unroll
-                for (int c = 1; c < kMaxCluster; ++c) {
-                    if (c < size && high >= 7) {
+                for (int j = 0; j < 8; ++j)
+                    if (high - j >= mine_from) mine[j] = shared.histogram[high - j];
+            } else if (high >= mine_from) {
+#pragma unroll
+                for (int c = 0; c < kMaxCluster; ++c) {
+                    if (c < size) {
                         const uint4* other = reinterpret_cast<const uint4*>(cluster.map_shared_rank(shared.histogram, (rank + c) % size) + high - 7);
                         const uint4 a = other[0], b = other[1];
                         mine[7] += a.x; mine[6] += a.y; mine[5] += a.z; mine[4] += a.w;
@@ -168,17 +175,36 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
             __syncthreads();
             uint32_t running = inclusive - sum;
             for (int w = 0; w < warp; ++w) running += shared.greater[w];
+            int owner = 0;
+            uint32_t ahead = 0u;  // candidates in the slices above the owner's
+            if (size > 1) {
+                if (tid == threads - 1) shared.slice = running + sum;
+                cluster.sync();
+                const uint32_t slice = lane < size ? *cluster.map_shared_rank(&shared.slice, lane % size) : 0u;
+                uint32_t upto = slice;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (running < missing && running + mine[j] >= missing) {
-                    shared.digit = high - j;
-                    shared.above = running;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t other = __shfl_up_sync(kFullMask, upto, o);
+                    if (lane >= o) upto += other;
                 }
-                running += mine[j];
+                owner = __ffs(__ballot_sync(kFullMask, upto >= missing)) - 1;
+                ahead = __shfl_sync(kFullMask, upto - slice, owner);
             }
-            meet();  // the digit is known here, and every CTA has read the histograms
-            prefix = (prefix << (kShift[pass] - shift)) | shared.digit;
-            missing -= shared.above;
+            if (rank == owner) {
+                running += ahead;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (running < missing && running + mine[j] >= missing) {
+                        shared.digit = high - j;
+                        shared.above = running;
+                    }
+                    running += mine[j];
+                }
+            }
+            meet();  // the digit is known, and every CTA has read the histograms
+            const uint32_t digit = *cluster.map_shared_rank(&shared.digit, owner), above = *cluster.map_shared_rank(&shared.above, owner);
+            prefix = (prefix << (kShift[pass] - shift)) | digit;
+            missing -= above;
         }
         // candidates above the threshold are kept, and the first `missing` equal to it; a warp takes a contiguous stretch
         const int stretch = ((to - from + warps - 1) / warps + 31) & ~31;
@@ -269,12 +295,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
     };
     int item = rank * warps + warp, stage = 0;
     Place now, then;
-    find(now, item, token_of(item));
-    int token = token_of(item + wave);
+    const int first_token = token_of(item), next_token = token_of(item + wave);
+    int token = token_of(item + 2 * wave);
+    find(now, item, first_token);
+    find(then, item + wave, next_token);
     load_scales(now, item);
     load_codes(now, item, 0);
-    find(then, item + wave, token);
-    token = token_of(item + 2 * wave);
     load_scales(then, item + wave);
     for (int done = 0; done < items; done += wave) {
         Place later;
@@ -283,6 +309,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
         token = token_of(item + 3 * wave);
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();
+        // (relaxed: the sources have arrived in shared memory, and nothing that was written is handed on)
+        if (size > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         uint32_t amax = 0u;
         const uint4* codes = staged + stage * P * kRow + lane;
 #pragma unroll
@@ -304,7 +332,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
         const float fresh = amax != 0u ? block_scale<INT8>(amax) : 1.f;
         const float own_ratio = now.scale * (1.f / fresh);
         const bool exact = __all_sync(kFullMask, lane >= now.count || moves_exactly(own_ratio));
-        meet();  // every source of this wave has been read
+        if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every source of this wave has been read
+        else __syncthreads();
         const bool write = valid(now.to);
         const int64_t page = static_cast<int64_t>(now.to) * v.kv_heads + head, plane_page = (item & 1) * v.num_blocks * v.kv_heads + page;
 #pragma unroll
