@@ -6,6 +6,8 @@ Follows the arithmetic of the reference's cache hooks without vLLM
 block costs the sum of every owner's page (packed owners: 2 planes x heads x block_size x page_width bytes; native
 bf16 owners: 2 x heads x block_size x head_dim x 2 bytes), the pool holds `budget // bytes_per_block` blocks, and it
 must hold more than one full-length sequence (`ceil(max_model_len / block_size)`) because block 0 is the null block.
+Owners that keep their KV in 8 bits (block_cache.BlockCache, not part of the reference) cost 2 planes x heads x (block_size x
+head_dim + 4 bytes of scale), and 4 bytes for each token and head more where accumulated attention weights are kept.
 """
 
 from __future__ import annotations
@@ -35,14 +37,25 @@ class OwnerSpec:
     head_dim: int
     block_size: int
     records: Optional[Tuple[Tuple[int, int], ...]] = None   # None = native bf16 KV
+    eight_bit: bool = False                                 # a block_cache.BlockCache (without records)
+    weights: bool = False                                   # with accumulated attention weights
+
+    def __post_init__(self) -> None:
+        if (self.eight_bit and self.records is not None) or (self.weights and not self.eight_bit):
+            raise ValueError("8-bit owners have no records, and only they keep attention weights")
 
     @property
     def page_bytes(self) -> int:
         """Bytes of one block of this owner, both planes (vLLM's `page_size_bytes`)."""
+        if self.eight_bit:
+            return self.heads * (2 * (self.block_size * self.head_dim + 4) + (4 * self.block_size if self.weights else 0))
         per_token = page_width(self.records, self.head_dim) if self.records is not None else 2 * self.head_dim
         return 2 * self.heads * self.block_size * per_token
 
     def cache_shape(self, num_blocks: int) -> Tuple[int, ...]:
+        """Shape of the cache tensor; of an 8-bit owner that of its codes."""
+        if self.eight_bit:
+            return (2, num_blocks, self.heads, self.block_size, self.head_dim)
         if self.records is None:
             return (2, num_blocks, self.block_size, self.heads, self.head_dim)
         return (2, num_blocks, self.heads, self.block_size, page_width(self.records, self.head_dim))

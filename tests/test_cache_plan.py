@@ -59,3 +59,16 @@ def test_kv_footprint_per_token():
     # 100 GB of KV at context 8192: 79 sequences packed against 15 native
     assert cp.sequences_that_fit(100 * 10**9, 8192, packed) == 79
     assert cp.sequences_that_fit(100 * 10**9, 8192, 786432) == 15
+
+
+def test_eight_bit_owners_share_the_block_space():
+    plain, counted = cp.OwnerSpec(8, 128, 16, eight_bit=True), cp.OwnerSpec(8, 128, 16, eight_bit=True, weights=True)
+    assert plain.cache_shape(10) == (2, 10, 8, 16, 128)
+    assert plain.page_bytes == 2 * 8 * (16 * 128 + 4) and counted.page_bytes == plain.page_bytes + 8 * 16 * 4
+    plan = cp.plan_cache({"packed": cp.OwnerSpec(8, 128, 16, G32), "eight": counted, "native": cp.OwnerSpec(8, 128, 16)}, 10**9, 4096)
+    assert plan.bytes_per_block == 2 * 8 * 16 * (200 + 128 + 256) + 2 * 8 * 4 + 8 * 16 * 4
+    assert plan.owner_bytes["eight"] == plan.num_blocks * counted.page_bytes
+    with pytest.raises(ValueError):
+        cp.OwnerSpec(8, 128, 16, G32, eight_bit=True)
+    with pytest.raises(ValueError):
+        cp.OwnerSpec(8, 128, 16, weights=True)

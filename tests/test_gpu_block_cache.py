@@ -325,6 +325,61 @@ def test_attention_of_many_requests():
     check_attention(cache, batch, query, accumulate=True)
 
 
+@pytest.mark.parametrize("requests,length,kv_heads,group,rows,dim,page,dtype,act", [
+    (1, 40001, 1, 8, 1, 128, 16, E4M3, torch.bfloat16),      # one sequence is cut into hundreds of pieces
+    (1, 20011, 3, 1, 1, 96, 32, INT8, torch.float16),
+    (5, 9001, 2, 4, 1, 64, 16, E4M3, torch.bfloat16),
+    (3, 7000, 2, 3, 7, 128, 16, INT8, torch.bfloat16),       # rows in two tiles of sixteen queries
+    (40, 800, 2, 2, 1, 128, 32, E4M3, torch.float16),
+])
+def test_attention_over_long_sequences(requests, length, kv_heads, group, rows, dim, page, dtype, act):
+    """Against float64 on the GPU, a head at a time."""
+    lengths = [max(rows, length - 97 * i) for i in range(requests)]
+    batch = Batch([rows] * requests, lengths, page, seed=length)
+    cache = make_cache(batch, kv_heads, page, dim, dtype, weights=True)
+    query = rows_like(rows * requests, kv_heads * group, dim, act, 3, 0.3)
+    out, lse, start = torch.zeros_like(query), torch.zeros(query.shape[:2], device=DEVICE), cache.weights.double()
+    for accumulate in (False, True):
+        cache.attention(query, out, *batch.meta, lse=lse, accumulate=accumulate)
+        cache.attention_status()
+        added = torch.zeros_like(start)
+        for r, n in enumerate(lengths):
+            ids = torch.tensor([b for b in batch.table[r] if b >= 0], device=DEVICE)
+            for h in range(kv_heads):
+                keys, values = ((cache.codes.view(torch.uint8)[plane, ids, h].view(dtype).double() * cache.scales[plane, ids, h].double()[:, None, None])
+                                .flatten(0, 1)[:n] for plane in range(2))
+                q = query[rows * r:rows * (r + 1), h * group:(h + 1) * group].double()
+                scores = torch.einsum("igd,td->igt", q, keys) * dim ** -0.5
+                hidden = torch.arange(n, device=DEVICE) > (n - rows + torch.arange(rows, device=DEVICE))[:, None]
+                scores = scores.masked_fill(hidden[:, None], float("-inf"))
+                w = torch.softmax(scores, 2)
+                want, magnitude = w @ values, w @ values.abs()
+                spread = (q.abs() @ keys.abs().T).amax(2) * dim ** -0.5
+                limit = block_oracle.tolerance(want, magnitude, spread, n, act, float(values.abs().max()))
+                got = out[rows * r:rows * (r + 1), h * group:(h + 1) * group].double()
+                assert torch.all((got - want).abs() <= limit)
+                got = lse[rows * r:rows * (r + 1), h * group:(h + 1) * group].double()
+                slack = 2 * (dim + 8) * 2.0 ** -24 * spread + 2.0 ** -18 + 2.0 ** -22 * got.abs()
+                assert torch.all((got - torch.logsumexp(scores, 2)).abs() <= slack)
+                sums = torch.zeros(ids.numel() * page, dtype=torch.float64, device=DEVICE)
+                sums[:n] = w.sum((0, 1))
+                added[ids, h] = sums.reshape(-1, page)
+        if accumulate:
+            score = 2 * (dim + 8) * 2.0 ** -24 * 40.0 + 2.0 ** -17      # scores here add up to less than 40 in magnitude
+            assert float(spread.max()) < 40.0
+            assert torch.all((cache.weights.double() - start - added).abs() <= score * added + 2.0 ** -22 * (start + added))
+
+
+def test_attention_adds_up_the_weights_of_requests_that_share_blocks():
+    batch = Batch([1, 1], [48, 48], 16)
+    batch.table[1] = batch.table[0]
+    batch.meta = (batch.meta[0], batch.meta[1], ints(batch.table))
+    cache = make_cache(batch, 2, 16, 64, E4M3, weights=True)
+    cache.weights.zero_()
+    check_attention(cache, batch, rows_like(2, 4, 64, torch.bfloat16, 1, 0.3), accumulate=True)
+    assert abs(float(cache.weights.sum()) - 2 * 4) < 1e-4
+
+
 def test_attention_over_a_cache_beyond_32_bit_offsets():
     blocks, heads, dim = 70001, 16, 128                  # 4.6 GB of codes
     if torch.cuda.mem_get_info()[0] < 8 << 30:
@@ -396,7 +451,9 @@ def test_evict_of_special_weights(kind):
     same_cache(cache, oracle)
 
 
-@pytest.mark.parametrize("requests,length,budget", [(1, 20011, 5003), (40, 700, 300), (300, 60, 33)])
+@pytest.mark.parametrize("requests,length,budget", [(1, 20011, 5003), (40, 700, 300), (300, 60, 33),
+                                                    (1, 300007, 1000),      # more weights than eight CTAs hold
+                                                    (76, 17003, 5000)])     # more than one holds
 def test_evict_of_long_sequences_and_large_batches(requests, length, budget):
     batch = Batch([1] * requests, [length] * requests, 16, seed=1)
     cache = make_cache(batch, 2, 16, 64, INT8, weights=True)
@@ -486,6 +543,31 @@ def test_calls_are_captured_and_replayed_with_new_lengths():
             torch.cuda.synchronize()
             results.append([t.clone() for t in (cache.codes.view(torch.uint8), cache.scales, cache.weights, out, lse, kept, left)])
         assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_two_captured_graphs_are_replayed_at_once():
+    """Each graph has scratch memory of its own: replayed on two streams they give what they give alone."""
+    batch = Batch([1] * 6, [1500] * 6, 16)
+    cache = make_cache(batch, 2, 16, 128, INT8)
+    queries, outs, wants, graphs = [], [], [], []
+    for s in (1, 2):
+        queries.append(rows_like(6, 8, 128, torch.bfloat16, s, 0.2))
+        outs.append(torch.zeros_like(queries[-1]))
+        wants.append(torch.zeros_like(queries[-1]))
+        cache.attention(queries[-1], wants[-1], *batch.meta)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(4):
+                outs[-1].zero_()
+                cache.attention(queries[-1], outs[-1], *batch.meta)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, wants))
 
 
 def test_two_streams_share_nothing():
