@@ -690,18 +690,21 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 
 // Joins the pieces of the items that more than one span took part in.  At most one such item begins in a span; the CTAs of
 // row `part` of the grid take every gridDim.y-th of its queries, all of their warps on as few at a time as leave none out.
-template <typename C>
-__global__ void __launch_bounds__(kJoinWarps * 32) block_join_kernel(const BlockAttentionParams p) {
-    constexpr int D = C::D, kRows = C::kRows, kLanes = D / 4, kBatch = 8;
+// kBatch pieces are on their way to a warp at once: many where one item is cut into hundreds, few registers (and all CTAs
+// resident) where many are cut in two.
+template <typename C, int kBatch>
+__global__ void __launch_bounds__(kJoinWarps * 32, kBatch > 2 ? 2 : 6) block_join_kernel(const BlockAttentionParams p) {
+    constexpr int D = C::D, kRows = C::kRows, kLanes = D / 4;
     __shared__ float4 sums[kJoinWarps][kLanes];
     __shared__ float4 stats[kJoinWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     pdl_launch_dependents();
-    const int each = (p.spans + gridDim.x - 1) / gridDim.x, behind = min(p.spans, static_cast<int>(blockIdx.x + 1) * each);
-    for (int span = blockIdx.x * each; span < behind; ++span) {
+    const int each = (p.spans + gridDim.x - 1) / gridDim.x, first_span = blockIdx.x * each;  // at most 32
+    const bool is_cut = lane < each && first_span + lane < p.spans && p.cuts[first_span + lane].pieces != 0;
+    for (uint32_t cuts = __ballot_sync(kFullMask, is_cut); cuts != 0u; cuts &= cuts - 1u) {
+        const int span = first_span + __ffs(cuts) - 1;
         const BlockCut cut = p.cuts[span];
-        if (cut.pieces == 0) continue;
         const int queries = min(kRows, cut.queries), parts = gridDim.y;
         int together = 1;  // queries that the CTA works on at a time
         while (together < kJoinWarps && together * parts < queries) together *= 2;
@@ -850,7 +853,8 @@ cudaError_t launch(const BlockAttentionParams& p, cudaStream_t stream) {
     if ((err = describe_codes(p.v, D, &launch.map)) != cudaSuccess) return err;
     err = launch_chained(block_attention_kernel<C>, launch, dim3(static_cast<unsigned>(p.spans)), kThreads, C::kSmem, 1, programmatic, stream);
     if (err == cudaSuccess && !p.whole_items)
-        err = launch_chained(block_join_kernel<Config<D, INT8, NT, false>>, p, dim3(static_cast<unsigned>(p.join_ctas), static_cast<unsigned>(p.join_parts)), kJoinWarps * 32, 0, 1, programmatic, stream);
+        err = launch_chained(p.join_parts > 2 ? block_join_kernel<Config<D, INT8, NT, false>, 8> : block_join_kernel<Config<D, INT8, NT, false>, 2>, p,
+                             dim3(static_cast<unsigned>(p.join_ctas), static_cast<unsigned>(p.join_parts)), kJoinWarps * 32, 0, 1, programmatic, stream);
     if (err == cudaSuccess && SCORES) {
         const unsigned parts = static_cast<unsigned>(std::min(64, (p.max_len + 4 * kThreads - 1) / (4 * kThreads)));
         if (parts > 0)

@@ -757,10 +757,10 @@ static int block_attention_params(const RqBlockAttentionArgs* a, rq::BlockAttent
             p->scores = reinterpret_cast<float*>(base + partials + cuts + lse);
         }
     }
-    // Where there are few items each can have many pieces: every query is joined by a CTA of its own, and fewer CTAs look for
-    // the items, neighbouring spans each (items of many pieces begin far apart).
+    // Where there are few items each can have many pieces: every query is joined by a CTA of its own, and a CTA looks for the
+    // items of sixteen neighbouring spans (items of many pieces begin far apart).
     p->join_parts = items * 8 <= current_sm_count() ? 8 : 2;
-    p->join_ctas = p->join_parts == 8 && p->spans > current_sm_count() ? current_sm_count() : p->spans;
+    p->join_ctas = p->join_parts == 8 ? (p->spans + 15) / 16 : p->spans;
     return RQ_OK;
 }
 
