@@ -3,6 +3,7 @@ ResidualQuant-style KV-cache compression for looped Transformers, behind the ref
 
     from residualquant_b200 import _cuda            # attention(...), quantize(...): reference signatures
     from residualquant_b200.rotation import register_rotation
+    from residualquant_b200.block_cache import BlockCache   # 8-bit cache of owners that are not residual-coded
 """
 
 __version__ = "0.1.0"
