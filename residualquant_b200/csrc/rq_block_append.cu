@@ -45,12 +45,6 @@ __device__ __noinline__ uint2 encode8(uint4 x, float inverse, bool fp16) {
 
 // Largest of two pairs' 16-bit magnitudes, pair by pair.
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b & 0x7fff7fffu); }
-// 16-bit magnitude bits, of finite values only.
-__device__ __forceinline__ uint32_t finite_or_zero(uint32_t pair, uint32_t infinity) {
-    const uint32_t low = pair & 0x7fffu, high = (pair >> 16) & 0x7fffu;
-    return max(low < infinity ? low : 0u, high < infinity ? high : 0u);
-}
-
 template <int D, int P, bool INT8>
 __global__ void __launch_bounds__(kAppendWarps * 32) block_append_kernel(const BlockAppendParams p) {
     constexpr int kRow = D / 8;             // pieces of eight channels in a row

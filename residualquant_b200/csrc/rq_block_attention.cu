@@ -215,6 +215,16 @@ __device__ __forceinline__ Place find_place(const BlockAttentionParams& p, Place
     return place;
 }
 
+// A query's row in its request and its head in the group (mostly there is one row, and no division).
+struct RowHead {
+    int row, head;
+};
+__device__ __forceinline__ RowHead row_and_head(int query, int group) {
+    if (query < group) return {0, query};
+    const int row = query / group;
+    return {row, query - row * group};
+}
+
 // Writes one query's finished output channels (four of them) and, from one thread of it, its lse.
 __device__ __forceinline__ void write_output(const BlockAttentionParams& p, int row, int head, int D, int channel, float4 o, float m,
                                              float l, float M) {
@@ -270,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
     // Windows: lane i holds the page id of the warp's unit 32 w + i (-1: none, or outside the cache) and its scales, and of
     // the window after it the ids from the window's start on and the scales from its middle on.
     int ids, ids_next;
-    float key_scales, value_scales, key_scales_next, value_scales_next;  // the latter as log2
+    float key_scales, value_scales, key_scales_next, value_scales_next;
     auto window = [&](int first) {
         const int unit = first + lane;
         const int id = unit < units ? v.block_table[static_cast<int64_t>(r) * v.table_stride + ((token_begin + (warp + unit * kWarps) * kUnit) >> page_shift)] : -1;
@@ -330,17 +340,17 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
         if ((unit & 31) == 0) {
             if (unit == 0) {
                 key_scales = scale(ids, 0);
-                value_scales = log2_fast(scale(ids, 1));
+                value_scales = scale(ids, 1);
             }
         } else if ((unit & 31) == 16) {
             key_scales_next = scale(ids_next, 0);
-            value_scales_next = log2_fast(scale(ids_next, 1));
+            value_scales_next = scale(ids_next, 1);
         }
     };
     auto describe = [&](int unit, int to) {
         if (unit >= units) return;
         const int id = __shfl_sync(kFullMask, ids, unit & 31);
-        const float k = __shfl_sync(kFullMask, key_scales, unit & 31), log_v = __shfl_sync(kFullMask, value_scales, unit & 31);
+        const float k = __shfl_sync(kFullMask, key_scales, unit & 31), log_v = log2_fast(__shfl_sync(kFullMask, value_scales, unit & 31));
         const int count = id >= 0 ? min(kUnit, token_end - (token_begin + (warp + unit * kWarps) * kUnit)) : 0;
         if (lane == 0) info[to] = make_float4(k, log_v, __int_as_float(count), 0.f);
     };
@@ -350,7 +360,8 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
         for (int i = tid; i < kRows * (D / 8); i += kThreads) {
             const int query = query0 + i / (D / 8);
             const bool real = query < q.queries;
-            const int row = real ? q.first + query / p.group : q.first, query_head = head * p.group + (real ? query % p.group : 0);
+            const RowHead at = row_and_head(real ? query : 0, p.group);
+            const int row = q.first + at.row, query_head = head * p.group + at.head;
             copy16_or_zero(static_cast<uint32_t>(__cvta_generic_to_shared(smem + C::kOffQuery + i * 16)),
                            static_cast<const uint16_t*>(p.query) + row * p.query_stride + query_head * D + i % (D / 8) * 8, real);
         }
@@ -385,16 +396,18 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
                 raw[s][0] = two.x;
                 raw[s][1] = two.y;
             }
-            uint32_t amax = 0u;
+            // the largest magnitude, on the 16-bit patterns; infinities and NaN, if any, are left out one by one
+            uint32_t pairs = 0u;
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < kSteps; ++s) pairs = __vmaxu2(__vmaxu2(pairs, raw[s][0] & 0x7fff7fffu), raw[s][1] & 0x7fff7fffu);
+            uint32_t bits = max(pairs & 0xffffu, pairs >> 16);
+            const uint32_t infinity = p.fp16 ? 0x7c00u : 0x7f80u;
+            if (bits >= infinity) {
+                bits = 0u;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float2 f = activation2(raw[s][i], p.fp16);
-                    const uint32_t a = __float_as_uint(f.x) & 0x7fffffffu, b = __float_as_uint(f.y) & 0x7fffffffu;
-                    amax = max(amax, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
-                }
+                for (int s = 0; s < kSteps; ++s) bits = max(bits, max(finite_or_zero(raw[s][0], infinity), finite_or_zero(raw[s][1], infinity)));
             }
+            uint32_t amax = __float_as_uint(activation2(bits, p.fp16).x);
             amax = max(amax, __shfl_xor_sync(kFullMask, amax, 1));
             amax = max(amax, __shfl_xor_sync(kFullMask, amax, 2));
             // the largest magnitude goes to [2^14, 2^15): exact for everything down to 2^-39 of it
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
             for (int i = 0; i < 2; ++i) {
                 factor[n][i] = __shfl_sync(kFullMask, up, (2 * t + i) * 4) * p.scale_log2;
                 const int column = query0 + n * 8 + 2 * t + i;
-                limit[n][i] = column < q.queries ? max(0, min(q.tokens, q.before + column / p.group + 1)) : 0x7fffffff;
+                limit[n][i] = column < q.queries ? max(0, min(q.tokens, q.before + row_and_head(column, p.group).row + 1)) : 0x7fffffff;
                 least = min(least, limit[n][i]);
             }
         }
@@ -430,7 +443,8 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int column = query0 + n * 8 + 2 * t + i;
-                    const int64_t query_row = static_cast<int64_t>(q.first + column / p.group) * p.heads + head * p.group + column % p.group;
+                    const RowHead at = row_and_head(column, p.group);
+                    const int64_t query_row = static_cast<int64_t>(q.first + at.row) * p.heads + head * p.group + at.head;
                     score_at[n][i] = column < q.queries ? p.scores + query_row * p.score_stride : nullptr;
                 }
             }
@@ -668,7 +682,8 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
                     sum.w += part.w * share;
                 }
                 if (done_whole) {
-                    write_output(p, done_first + query / p.group, done_head * p.group + query % p.group, D, channel, sum, m_all, l_all, M_all);
+                    const RowHead at = row_and_head(query, p.group);
+                    write_output(p, done_first + at.row, done_head * p.group + at.head, D, channel, sum, m_all, l_all, M_all);
                 } else {
                     float* to = p.partials + (done_slot * kRows + n * 8 + column) * C::kSlot;
                     *reinterpret_cast<float4*>(to + channel) = sum;
@@ -763,7 +778,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kBatch > 2 ? 2 : 6) block_joi
             }
             if (mine == 0 && column < queries && lane < kLanes) {
                 const int query = cut.query0 + column;
-                write_output(p, cut.first + query / p.group, cut.head * p.group + query % p.group, D, lane * 4, sum, m, l, M);
+                const RowHead at = row_and_head(query, p.group);
+                write_output(p, cut.first + at.row, cut.head * p.group + at.head, D, lane * 4, sum, m, l, M);
             }
         }
     }

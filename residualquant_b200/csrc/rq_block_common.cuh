@@ -69,6 +69,12 @@ __device__ __forceinline__ float2 activation2(uint32_t pair, bool fp16) {
     return make_float2(bf16_bits_to_float(pair & 0xffffu), __uint_as_float(pair & 0xffff0000u));
 }
 
+// The larger 16-bit magnitude of a pair, of finite values only.
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t pair, uint32_t infinity) {
+    const uint32_t low = pair & 0x7fffu, high = (pair >> 16) & 0x7fffu;
+    return max(low < infinity ? low : 0u, high < infinity ? high : 0u);
+}
+
 __device__ __forceinline__ uint32_t pack_activation2(float a, float b, bool fp16) {
     if (fp16) {
         const __half2_raw raw = __half2_raw(__floats2half2_rn(a, b));
