@@ -68,11 +68,14 @@ struct Config {
     static_assert(8 * D * 4 <= kStage, "a warp's sums fit a stage");
     static constexpr int kOffInfo = kWarps * kStages * kStage;        // float4 [warps][stages]: K scale, log2 of V's, tokens
     static constexpr int kOffStat = kOffInfo + kWarps * kStages * 16; // float [warps][8][4]: m, l, M, the stage of the sums
-    static constexpr int kOffQuery = kOffStat + kWarps * 8 * 16;      // 16-bit [rows][D]: the next piece's queries
+    static constexpr int kOffQuery = kOffStat + kWarps * 8 * 16;      // 16-bit [buffers][rows][D]: a piece's queries
     // sixteen queries would take too many registers: their fp16 fragments stay in shared memory, [n][pair of steps][lane]
     static constexpr bool kSharedQueries = NT > 1;
-    static constexpr int kOffFragments = kOffQuery + kRows * D * 2;
-    static constexpr int kOffBarrier = kOffFragments + (kSharedQueries ? kRows * D * 2 : 0);  // uint64 [warps][stages]
+    // The next piece's queries come in while a slow warp may still take in this one's, unless all warps met in between, as they
+    // do over the shared fragments: two buffers, or one.
+    static constexpr int kQueryBytes = kRows * D * 2, kQueryBuffers = kSharedQueries ? 1 : 2;
+    static constexpr int kOffFragments = kOffQuery + kQueryBuffers * kQueryBytes;
+    static constexpr int kOffBarrier = kOffFragments + (kSharedQueries ? kQueryBytes : 0);  // uint64 [warps][stages]
     static constexpr int kOffPlace = kOffBarrier + kWarps * kStages * 8;
     static constexpr int kSmem = kOffPlace + 64;
     static constexpr int kSlot = D + 4;                               // floats a query's partial result takes
@@ -355,14 +358,16 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
         if (lane == 0) info[to] = make_float4(k, log_v, __int_as_float(count), 0.f);
     };
     int stage = 0;       // of the next unit to be used
+    uint8_t* queries = smem + C::kOffQuery;  // of the piece that was set off last
     auto set_off = [&]() {
+        if constexpr (C::kQueryBuffers == 2) queries = queries == smem + C::kOffQuery ? queries + C::kQueryBytes : smem + C::kOffQuery;
         // the piece's queries, ahead of the queue of cache copies (rows behind the item's last are zeros)
         for (int i = tid; i < kRows * (D / 8); i += kThreads) {
             const int query = query0 + i / (D / 8);
             const bool real = query < q.queries;
             const RowHead at = row_and_head(real ? query : 0, p.group);
             const int row = q.first + at.row, query_head = head * p.group + at.head;
-            copy16_or_zero(static_cast<uint32_t>(__cvta_generic_to_shared(smem + C::kOffQuery + i * 16)),
+            copy16_or_zero(static_cast<uint32_t>(__cvta_generic_to_shared(queries + i * 16)),
                            static_cast<const uint16_t*>(p.query) + row * p.query_stride + query_head * D + i % (D / 8) * 8, real);
         }
         commit_copies();
@@ -392,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 const int channel = t * (D / 4) + s * 4;
-                const uint2 two = *reinterpret_cast<const uint2*>(smem + C::kOffQuery + ((n * 8 + g) * D + channel) * 2);
+                const uint2 two = *reinterpret_cast<const uint2*>(queries + ((n * 8 + g) * D + channel) * 2);
                 raw[s][0] = two.x;
                 raw[s][1] = two.y;
             }

@@ -309,7 +309,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
         token = token_of(item + 3 * wave);
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();
-        // (relaxed: the sources have arrived in shared memory, and nothing that was written is handed on)
+        // The vote has every lane's scale and weight arrive as well, before any warp may write to where they came from.
+        const bool odd = __any_sync(kFullMask, now.scale != now.scale || now.moved != now.moved);
+        // (relaxed: the sources have arrived, and nothing that was written is handed on)
         if (size > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         uint32_t amax = 0u;
         const uint4* codes = staged + stage * P * kRow + lane;
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
         amax = __reduce_max_sync(kFullMask, amax);
         const float fresh = amax != 0u ? block_scale<INT8>(amax) : 1.f;
         const float own_ratio = now.scale * (1.f / fresh);
-        const bool exact = __all_sync(kFullMask, lane >= now.count || moves_exactly(own_ratio));
+        const bool exact = !odd && __all_sync(kFullMask, lane >= now.count || moves_exactly(own_ratio));
         if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every source of this wave has been read
         else __syncthreads();
         const bool write = valid(now.to);
