@@ -315,6 +315,16 @@ def test_attention_of_strided_rows():
     assert torch.equal(again, plain)
 
 
+def test_attention_writes_over_its_queries():
+    batch = Batch([1, 3, 1], [700, 90, 2500], 16)
+    cache = make_cache(batch, 2, 16, 128, INT8)
+    query = rows_like(5, 8, 128, torch.bfloat16, 6, 0.2)
+    want = torch.zeros_like(query)
+    cache.attention(query, want, *batch.meta)
+    cache.attention(query, query, *batch.meta)
+    assert torch.equal(query, want)
+
+
 def test_attention_of_many_requests():
     rng = random.Random(1)
     lengths = [rng.choice([0, 1, 5, 16, 30, 64, 100]) for _ in range(700)]
