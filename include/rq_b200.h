@@ -368,14 +368,14 @@ typedef struct RqBlockAttentionArgs {
     float softmax_scale;
     float* lse;         /* fp32 [num_rows][heads], natural logarithm, or NULL */
     int32_t max_seq_len; /* upper bound of seq_lens for this call, 0 = the page table's width; tokens from it on are not
-                            seen.  It bounds an accumulating call's workspace, and up to 256 one launch less is needed */
+                            seen.  It bounds an accumulating call's workspace, and up to 512 one launch less is needed */
     void* workspace;    /* rq_block_attention_workspace_bytes() bytes, 256-byte aligned (NULL for 0 bytes); no initialisation needed */
     size_t workspace_bytes;
     void* stream;
     int32_t flags;      /* RQ_FLAG_SERIAL_LAUNCH */
 } RqBlockAttentionArgs;
 /* Scratch one rq_block_attention call needs; workspace and workspace_bytes of the arguments are not looked at.  0 where it
- * needs none (up to 256 tokens, nothing accumulated) or the arguments are not valid. */
+ * needs none (short page tables, nothing accumulated) or the arguments are not valid. */
 size_t rq_block_attention_workspace_bytes(const RqBlockAttentionArgs* args);
 int32_t rq_block_attention(const RqBlockAttentionArgs* args);
 /* Synchronizes `stream`: RQ_OK, or RQ_ERR_DEVICE_TIMEOUT if a bounded wait inside a block attention kernel ever gave up

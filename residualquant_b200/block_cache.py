@@ -153,7 +153,7 @@ class BlockCache:
 
         `accumulate` adds every token's softmax weight, summed over the rows and over the query heads of its KV head, to the
         cache's `weights`.  Such a call needs scratch memory for rows x heads x `max_seq_len` scores.  `max_seq_len` (default: the
-        block table's width) must be no smaller than any of `seq_lens`: tokens behind it are not seen; up to 256 saves a launch."""
+        block table's width) must be no smaller than any of `seq_lens`: tokens behind it are not seen; up to 512 saves a launch."""
         heads = query.size(1) if query.dim() == 3 else 0
         query_stride, output_stride = self._rows(query, heads, "query"), self._rows(output, heads, "output")
         rows = query.size(0)

@@ -199,7 +199,7 @@ __device__ __forceinline__ Place find_place(const BlockAttentionParams& p, Place
         if (w < warp) running += shared.warp_sums[w];
         place.total += shared.warp_sums[w];
     }
-    place.span = max(static_cast<int64_t>(p.min_span), (place.total + p.spans - 1) / p.spans);
+    place.span = max(static_cast<int64_t>(1), (place.total + p.spans - 1) / p.spans);
     const int64_t target = at * place.span;
     if (running <= target && target < running + sum) {
         for (int r = lo; r < hi; ++r) {
@@ -899,9 +899,7 @@ cudaError_t block_attention_status(cudaStream_t stream, int* status) {
     return err == cudaSuccess ? cudaStreamSynchronize(stream) : err;
 }
 
-// Items of up to four chunks are not cut: a CTA takes about as long for them as for the join of two halves.
-bool block_attention_whole(int tokens) { return tokens <= 4 * kChunk; }
-int64_t block_attention_units(int tokens) { return block_attention_whole(tokens) ? 1 : (tokens + kChunk - 1) / kChunk + kItemCost; }
+int64_t block_attention_units(int tokens) { return (tokens + kChunk - 1) / kChunk + kItemCost; }
 int block_attention_resident(int query_tiles) { return resident(query_tiles); }
 
 cudaError_t launch_block_attention(const BlockAttentionParams& p, int head_dim, int int8, cudaStream_t stream) {

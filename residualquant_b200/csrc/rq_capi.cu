@@ -737,9 +737,12 @@ static int block_attention_params(const RqBlockAttentionArgs* a, rq::BlockAttent
     p->query_tiles = rows_each * p->group <= 8 ? 1 : 2;
     // One span for each resident CTA, fewer where the batch cannot have that many units of work.
     const int64_t items = (static_cast<int64_t>(a->num_rows) * p->group / (8 * p->query_tiles) + a->batch.num_requests) * a->cache.kv_heads;
-    const int64_t units = items * rq::block_attention_units(p->max_len), resident = static_cast<int64_t>(rq::block_attention_resident(p->query_tiles)) * current_sm_count();
-    p->min_span = 1;
-    p->whole_items = rq::block_attention_whole(p->max_len) ? 1 : 0;
+    const int64_t resident = static_cast<int64_t>(rq::block_attention_resident(p->query_tiles)) * current_sm_count();
+    // Short items are not cut, which saves the join's launch; longer ones neither where there is about one for each CTA.  (A
+    // call in a graph, 8 heads, cut / not cut: 16 x 400 tokens 12.6 / 9.1 us, 16 x 800 14.0 / 13.4, 4 x 800 10.8 / 13.1, 64 x 800
+    // 22.8 / 19.3, 128 x 800 36.1 / 37.3, 32 x 1500 21.9 / 25.8.)
+    p->whole_items = p->max_len <= 512 || (p->max_len <= 1024 && items >= current_sm_count() && 4 * items <= 5 * resident) ? 1 : 0;
+    const int64_t units = items * (p->whole_items ? 1 : rq::block_attention_units(p->max_len));
     p->spans = static_cast<int>(units > resident ? resident : units);
     // workspace: unfinished pieces, then what an accumulating call leaves for its last launch
     const size_t partials = p->whole_items ? 0 : round_up(static_cast<size_t>(2) * p->spans * rq::block_attention_slot_floats(a->cache.head_dim, p->query_tiles) * sizeof(float), 256);

@@ -163,7 +163,7 @@ struct BlockAttentionParams {
     float scale_log2;        // softmax scale * log2(e)
     float* lse;              // or nullptr
     int query_tiles;         // eights of queries that a CTA takes together
-    int spans, min_span;     // CTAs that the work is cut for, and the fewest units each takes
+    int spans;               // CTAs that the work is cut for
     int whole_items;         // items are not cut: no join
     float* partials;         // workspace [2 * spans][8 * query_tiles][head_dim + 4]: value sums, m, l, M of unfinished pieces
     BlockCut* cuts;          // workspace [spans]
@@ -173,8 +173,7 @@ struct BlockAttentionParams {
     int64_t score_stride;
     int programmatic_launch;
 };
-int64_t block_attention_units(int tokens);  // of work that an item of this many tokens is counted as
-bool block_attention_whole(int tokens);     // whether items of up to this many tokens are not cut
+int64_t block_attention_units(int tokens);  // of work that an item of this many tokens is counted as, where items are cut
 int block_attention_resident(int query_tiles);  // CTAs on a multiprocessor
 int block_attention_slot_floats(int head_dim, int query_tiles);
 cudaError_t block_attention_status(cudaStream_t stream, int* status);  // of the current device; synchronizes
