@@ -16,9 +16,9 @@ A cached value is code * scale.  `append` and `evict` write scales that are powe
 largest finite magnitude into the codes' range (448 for float8_e4m3fn, 127 for int8); infinities saturate and NaN is stored as 0.
 `attention` reads any positive finite scales and finite codes.
 
-Nothing here synchronizes, and every call can be captured in a CUDA graph.  Calls go to the current stream of the cache's device;
-scratch memory is taken from PyTorch's allocator for each call, so calls on different streams share none.  Rejected arguments
-raise RuntimeError.
+Nothing here but `attention_status` synchronizes, and every other call can be captured in a CUDA graph.  Calls go to the current
+stream of the cache's device; scratch memory is taken from PyTorch's allocator for each call, so calls on different streams share
+none.  Rejected arguments raise RuntimeError.
 """
 
 from __future__ import annotations
