@@ -12,9 +12,13 @@
 //
 // Softmax in one pass, base 2: x = score * log2(e), l = sum 2^(x - m), O = sum 2^(x + log2(v scale) - M + 7) * code with
 // references m and M that are raised only when a token exceeds them by 2^8 (any thread of the warp sees one), so most tokens
-// need no reduction across threads.  Statistics and sums are fp32; the weights that multiply V are fp16 (11 bits, at most
-// 2^15, exact to 2^-31 of the largest one below that).  Separate references for l and O keep blocks of tiny value scales
-// from losing either.
+// need no reduction across threads.  Statistics and sums are fp32.  Separate references for l and O keep blocks of tiny value
+// scales from losing either.  A weight that multiplies V is the sum of two fp16 numbers, its upper eleven bits and the rest
+// (at most 2^15; off by 2^-22 of itself, or by 2^-31 of the largest one where that is more), with a product for each.  An item
+// of up to four queries has both in one instruction: its queries stand in columns 0..3 and again in columns 4..7, where the
+// rests are, and the two sums are added up in the end.  (One fp16 number for each weight left sums off by up to 2^-12 of
+// their terms' magnitude, which shows where they nearly cancel.  The rests cost 0 to 2 % with up to four queries, 64 sequences x 8192 tokens x 16 heads; 4 % with five
+// rows, 92 to 96 us; with sixteen queries, 64 x 8192 x 128/8 heads, 224 became 257 us.)
 //
 // Memory bound: 2 D bytes for each cached token and KV head.  All items' tokens, in chunks of kChunk and kItemCost chunks
 // more for each item, are laid end to end and cut into equal spans, one for each CTA (four per SM, three with sixteen queries;
@@ -27,6 +31,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "rq_block_common.cuh"
 
@@ -118,6 +123,13 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// A float's upper eleven bits: exact in fp16 from 2^-14 on.
+__device__ __forceinline__ float upper_bits(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+// x = from - x, in threads where `here`.
+__device__ __forceinline__ void subtract_where(float (&x)[4], const float (&from)[4], bool here) {
+    asm("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %8, 0;\n\t@p sub.f32 %0, %4, %0;\n\t@p sub.f32 %1, %5, %1;\n\t@p sub.f32 %2, %6, %2;\n\t@p sub.f32 %3, %7, %3;\n\t}"
+        : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]) : "f"(from[0]), "f"(from[1]), "f"(from[2]), "f"(from[3]), "r"(static_cast<int>(here)));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -358,12 +370,15 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
         if (lane == 0) info[to] = make_float4(k, log_v, __int_as_float(count), 0.f);
     };
     int stage = 0;       // of the next unit to be used
+    // The query that a column of the products stands for (up to four queries stand there twice).
+    auto folded = [&]() { return NT == 1 && q.queries - query0 <= 4; };
+    auto query_of = [&](int column) { return folded() ? column & 3 : column; };
     uint8_t* queries = smem + C::kOffQuery;  // of the piece that was set off last
     auto set_off = [&]() {
         if constexpr (C::kQueryBuffers == 2) queries = queries == smem + C::kOffQuery ? queries + C::kQueryBytes : smem + C::kOffQuery;
         // the piece's queries, ahead of the queue of cache copies (rows behind the item's last are zeros)
         for (int i = tid; i < kRows * (D / 8); i += kThreads) {
-            const int query = query0 + i / (D / 8);
+            const int query = query0 + query_of(i / (D / 8));
             const bool real = query < q.queries;
             const RowHead at = row_and_head(real ? query : 0, p.group);
             const int row = q.first + at.row, query_head = head * p.group + at.head;
@@ -434,12 +449,13 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 factor[n][i] = __shfl_sync(kFullMask, up, (2 * t + i) * 4) * p.scale_log2;
-                const int column = query0 + n * 8 + 2 * t + i;
+                const int column = query0 + query_of(n * 8 + 2 * t + i);
                 limit[n][i] = column < q.queries ? max(0, min(q.tokens, q.before + row_and_head(column, p.group).row + 1)) : 0x7fffffff;
                 least = min(least, limit[n][i]);
             }
         }
         least = __reduce_min_sync(kFullMask, least);
+        const bool fold = folded(), fold_lower = fold && t >= 2;
         if constexpr (C::kSharedQueries) __syncthreads();
         float* score_at[NT][2];
         if constexpr (C::kScores) {
@@ -470,178 +486,193 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) describe(i, stage + i < kStages ? stage + i : stage + i - kStages);
-        for (int unit = 0; unit < units; ++unit) {
-            const int free_stage = stage == 0 ? kStages - 1 : stage - 1;  // the one that the unit before was in
-            __syncwarp();                                                 // no lane reads it any more
-            produce(unit + kStages - 1, free_stage);
-            describe(unit + kStages - 1, free_stage);
-            uint32_t polls = 0;
-            while (!barrier_done(barriers + stage * 8, phases >> stage & 1u) && !failed) failed = ++polls > kWaitLimit;
-            phases ^= 1u << stage;
-            const uint8_t* keys = ring + stage * C::kStage;
-            const uint8_t* values = keys + C::kPlane;
-            const float4 about = info[stage];
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-            const int token0 = token_begin + (warp + unit * kWarps) * kUnit;
-            const int count = __float_as_int(about.z);
+        auto take_units = [&](auto folded_columns) {
+            constexpr bool kFold = decltype(folded_columns)::value;
+            for (int unit = 0; unit < units; ++unit) {
+                const int free_stage = stage == 0 ? kStages - 1 : stage - 1;  // the one that the unit before was in
+                __syncwarp();                                                 // no lane reads it any more
+                produce(unit + kStages - 1, free_stage);
+                describe(unit + kStages - 1, free_stage);
+                uint32_t polls = 0;
+                while (!barrier_done(barriers + stage * 8, phases >> stage & 1u) && !failed) failed = ++polls > kWaitLimit;
+                phases ^= 1u << stage;
+                const uint8_t* keys = ring + stage * C::kStage;
+                const uint8_t* values = keys + C::kPlane;
+                const float4 about = info[stage];
+                stage = stage + 1 == kStages ? 0 : stage + 1;
+                const int token0 = token_begin + (warp + unit * kWarps) * kUnit;
+                const int count = __float_as_int(about.z);
 
-            // scores
-            float x[NT][4], x_odd[NT][4];  // two sums, so that half the products wait for one another
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[n][i] = x_odd[n][i] = 0.f;
-            }
-            uint32_t low[kSteps], high[kSteps];  // K words of tokens g and g + 8
-            if constexpr (D == 128) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint4 a = *reinterpret_cast<const uint4*>(keys + place<D>(g, 2 * t + h));
-                    const uint4 b = *reinterpret_cast<const uint4*>(keys + place<D>(g + 8, 2 * t + h));
-                    low[4 * h] = a.x; low[4 * h + 1] = a.y; low[4 * h + 2] = a.z; low[4 * h + 3] = a.w;
-                    high[4 * h] = b.x; high[4 * h + 1] = b.y; high[4 * h + 2] = b.z; high[4 * h + 3] = b.w;
-                }
-            } else if constexpr (D == 64) {
-                const uint4 a = *reinterpret_cast<const uint4*>(keys + place<D>(g, t));
-                const uint4 b = *reinterpret_cast<const uint4*>(keys + place<D>(g + 8, t));
-                low[0] = a.x; low[1] = a.y; low[2] = a.z; low[3] = a.w;
-                high[0] = b.x; high[1] = b.y; high[2] = b.z; high[3] = b.w;
-            } else {
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    if (s & 1) continue;
-                    const uint2 a = *reinterpret_cast<const uint2*>(keys + g * 96 + t * 24 + s * 4);
-                    const uint2 b = *reinterpret_cast<const uint2*>(keys + (g + 8) * 96 + t * 24 + s * 4);
-                    low[s] = a.x; low[s + 1] = a.y;
-                    high[s] = b.x; high[s + 1] = b.y;
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < kSteps; s += 2) {
-                uint32_t a[4], b[4];
-                to_half<C::kInt8>(low[s], a[0], a[2]);
-                to_half<C::kInt8>(high[s], a[1], a[3]);
-                to_half<C::kInt8>(low[s + 1], b[0], b[2]);
-                to_half<C::kInt8>(high[s + 1], b[1], b[3]);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if constexpr (C::kSharedQueries) {
-                        const uint4 f = fragments[(n * kSteps + s) / 2 * 32];
-                        mma(x[n], a, f.x, f.y);
-                        mma(x_odd[n], b, f.z, f.w);
-                    } else {
-                        mma(x[n], a, qf[n][s][0], qf[n][s][1]);
-                        mma(x_odd[n], b, qf[n][s + 1][0], qf[n][s + 1][1]);
-                    }
-                }
-            }
-            const float value_scale = about.y;
-            const bool masked = count < kUnit || token0 + kUnit > least;
-            bool raise = false;
-            float top[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[n][i] = (x[n][i] + x_odd[n][i]) * (about.x * factor[n][i & 1]);
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int token = g + (i >> 1) * 8;
-                        if (token >= count || token0 + token >= limit[n][i & 1]) x[n][i] = -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    top[n][i] = fmaxf(x[n][i], x[n][i + 2]);
-                    raise = raise || top[n][i] > m[n][i] + kSlack || top[n][i] + value_scale > M[n][i] + kSlack;
-                }
-            }
-            if constexpr (C::kScores) {
+                // scores
+                float x[NT][4], x_odd[NT][4];  // two sums, so that half the products wait for one another
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int token = token0 + g + (i >> 1) * 8;
-                        if (score_at[n][i & 1] != nullptr && token < limit[n][i & 1]) score_at[n][i & 1][token] = x[n][i];
+                    for (int i = 0; i < 4; ++i) x[n][i] = x_odd[n][i] = 0.f;
+                }
+                uint32_t low[kSteps], high[kSteps];  // K words of tokens g and g + 8
+                if constexpr (D == 128) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint4 a = *reinterpret_cast<const uint4*>(keys + place<D>(g, 2 * t + h));
+                        const uint4 b = *reinterpret_cast<const uint4*>(keys + place<D>(g + 8, 2 * t + h));
+                        low[4 * h] = a.x; low[4 * h + 1] = a.y; low[4 * h + 2] = a.z; low[4 * h + 3] = a.w;
+                        high[4 * h] = b.x; high[4 * h + 1] = b.y; high[4 * h + 2] = b.z; high[4 * h + 3] = b.w;
+                    }
+                } else if constexpr (D == 64) {
+                    const uint4 a = *reinterpret_cast<const uint4*>(keys + place<D>(g, t));
+                    const uint4 b = *reinterpret_cast<const uint4*>(keys + place<D>(g + 8, t));
+                    low[0] = a.x; low[1] = a.y; low[2] = a.z; low[3] = a.w;
+                    high[0] = b.x; high[1] = b.y; high[2] = b.z; high[3] = b.w;
+                } else {
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) {
+                        if (s & 1) continue;
+                        const uint2 a = *reinterpret_cast<const uint2*>(keys + g * 96 + t * 24 + s * 4);
+                        const uint2 b = *reinterpret_cast<const uint2*>(keys + (g + 8) * 96 + t * 24 + s * 4);
+                        low[s] = a.x; low[s + 1] = a.y;
+                        high[s] = b.x; high[s + 1] = b.y;
                     }
                 }
-            }
-            if (__any_sync(kFullMask, raise)) {
+#pragma unroll
+                for (int s = 0; s < kSteps; s += 2) {
+                    uint32_t a[4], b[4];
+                    to_half<C::kInt8>(low[s], a[0], a[2]);
+                    to_half<C::kInt8>(high[s], a[1], a[3]);
+                    to_half<C::kInt8>(low[s + 1], b[0], b[2]);
+                    to_half<C::kInt8>(high[s + 1], b[1], b[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if constexpr (C::kSharedQueries) {
+                            const uint4 f = fragments[(n * kSteps + s) / 2 * 32];
+                            mma(x[n], a, f.x, f.y);
+                            mma(x_odd[n], b, f.z, f.w);
+                        } else {
+                            mma(x[n], a, qf[n][s][0], qf[n][s][1]);
+                            mma(x_odd[n], b, qf[n][s + 1][0], qf[n][s + 1][1]);
+                        }
+                    }
+                }
+                const float value_scale = about.y;
+                const bool masked = count < kUnit || token0 + kUnit > least;
+                bool raise = false;
+                float top[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[n][i] = (x[n][i] + x_odd[n][i]) * (about.x * factor[n][i & 1]);
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int token = g + (i >> 1) * 8;
+                            if (token >= count || token0 + token >= limit[n][i & 1]) x[n][i] = -INFINITY;
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float high_x = top[n][i];
+                        top[n][i] = fmaxf(x[n][i], x[n][i + 2]);
+                        raise = raise || top[n][i] > m[n][i] + kSlack || top[n][i] + value_scale > M[n][i] + kSlack;
+                    }
+                }
+                if constexpr (C::kScores) {
 #pragma unroll
-                        for (int step = 4; step < 32; step <<= 1) high_x = fmaxf(high_x, __shfl_xor_sync(kFullMask, high_x, step));
-                        const float m_new = fmaxf(m[n][i], high_x), M_new = fmaxf(M[n][i], high_x + value_scale);
-                        const float keep_l = exp2_fast(m[n][i] - m_new), keep_o = exp2_fast(M[n][i] - M_new);
-                        m[n][i] = m_new;
-                        M[n][i] = M_new;
-                        l[n][i] *= keep_l;
+                    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                        for (int s = 0; s < kSteps; ++s) {
-                            o[s][n][i] *= keep_o;
-                            o[s][n][i + 2] *= keep_o;
+                        for (int i = 0; i < 4; ++i) {
+                            const int token = token0 + g + (i >> 1) * 8;
+                            if (score_at[n][i & 1] != nullptr && token < limit[n][i & 1]) score_at[n][i & 1][token] = x[n][i];
+                        }
+                    }
+                }
+                if (__any_sync(kFullMask, raise)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float high_x = top[n][i];
+#pragma unroll
+                            for (int step = 4; step < 32; step <<= 1) high_x = fmaxf(high_x, __shfl_xor_sync(kFullMask, high_x, step));
+                            const float m_new = fmaxf(m[n][i], high_x), M_new = fmaxf(M[n][i], high_x + value_scale);
+                            const float keep_l = exp2_fast(m[n][i] - m_new), keep_o = exp2_fast(M[n][i] - M_new);
+                            m[n][i] = m_new;
+                            M[n][i] = M_new;
+                            l[n][i] *= keep_l;
+#pragma unroll
+                            for (int s = 0; s < kSteps; ++s) {
+                                o[s][n][i] *= keep_o;
+                                o[s][n][i + 2] *= keep_o;
+                            }
+                        }
+                    }
+                }
+                // weights, as fp16 and the fp16 of what that leaves over; the value scale goes into the exponent
+                uint32_t weight[NT][2], rest[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float w[4], upper[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        l[n][i & 1] += exp2_fast(x[n][i] - m[n][i & 1]);
+                        w[i] = exp2_fast(x[n][i] + (value_scale + kLift - M[n][i & 1]));
+                        upper[i] = upper_bits(w[i]);
+                    }
+                    if constexpr (kFold) {
+                        subtract_where(upper, w, fold_lower);
+                    } else {
+                        rest[n][0] = transpose8x8(pack_activation2(w[0] - upper[0], w[1] - upper[1], true));
+                        rest[n][1] = transpose8x8(pack_activation2(w[2] - upper[2], w[3] - upper[3], true));
+                    }
+                    weight[n][0] = transpose8x8(pack_activation2(upper[0], upper[1], true));
+                    weight[n][1] = transpose8x8(pack_activation2(upper[2], upper[3], true));
+                }
+                // value sums: tokens 2t, 2t + 1 (a[0], a[1]) and 2t + 8, 2t + 9 (a[2], a[3]); this thread's channels D/8 g ...
+                constexpr int kWords = D / 32;
+                uint32_t word[4][kWords];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int token = 2 * t + (i & 1) + (i >> 1) * 8;
+                    if constexpr (D == 128) {
+                        const uint4 a = *reinterpret_cast<const uint4*>(values + place<D>(token, g));
+                        word[i][0] = a.x; word[i][1] = a.y; word[i][2] = a.z; word[i][3] = a.w;
+                    } else if constexpr (D == 64) {
+                        const uint2 a = *reinterpret_cast<const uint2*>(values + place<D>(token, g >> 1) + (g & 1) * 8);
+                        word[i][0] = a.x; word[i][1] = a.y;
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < kWords; ++w) word[i][w] = *reinterpret_cast<const uint32_t*>(values + token * 96 + g * 12 + w * 4);
+                    }
+                }
+                if (count < kUnit) {  // whatever stands behind the last token, a weight of 0 must not meet it
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (2 * t + (i & 1) + (i >> 1) * 8 >= count) {
+#pragma unroll
+                            for (int w = 0; w < kWords; ++w) word[i][w] = 0u;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t a[4];
+                        to_half<C::kInt8>(__byte_perm(word[0][w], word[1][w], h == 0 ? 0x5140 : 0x7362), a[0], a[1]);
+                        to_half<C::kInt8>(__byte_perm(word[2][w], word[3][w], h == 0 ? 0x5140 : 0x7362), a[2], a[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma(o[2 * w + h][n], a, weight[n][0], weight[n][1]);
+                            if constexpr (!kFold) mma(o[2 * w + h][n], a, rest[n][0], rest[n][1]);
                         }
                     }
                 }
             }
-            // weights; the value scale goes into the exponent
-            uint32_t weight[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    l[n][i & 1] += exp2_fast(x[n][i] - m[n][i & 1]);
-                    w[i] = exp2_fast(x[n][i] + (value_scale + kLift - M[n][i & 1]));
-                }
-                weight[n][0] = transpose8x8(pack_activation2(w[0], w[1], true));
-                weight[n][1] = transpose8x8(pack_activation2(w[2], w[3], true));
-            }
-            // value sums: tokens 2t, 2t + 1 (a[0], a[1]) and 2t + 8, 2t + 9 (a[2], a[3]); this thread's channels D/8 g ...
-            constexpr int kWords = D / 32;
-            uint32_t word[4][kWords];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int token = 2 * t + (i & 1) + (i >> 1) * 8;
-                if constexpr (D == 128) {
-                    const uint4 a = *reinterpret_cast<const uint4*>(values + place<D>(token, g));
-                    word[i][0] = a.x; word[i][1] = a.y; word[i][2] = a.z; word[i][3] = a.w;
-                } else if constexpr (D == 64) {
-                    const uint2 a = *reinterpret_cast<const uint2*>(values + place<D>(token, g >> 1) + (g & 1) * 8);
-                    word[i][0] = a.x; word[i][1] = a.y;
-                } else {
-#pragma unroll
-                    for (int w = 0; w < kWords; ++w) word[i][w] = *reinterpret_cast<const uint32_t*>(values + token * 96 + g * 12 + w * 4);
-                }
-            }
-            if (count < kUnit) {  // whatever stands behind the last token, a weight of 0 must not meet it
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (2 * t + (i & 1) + (i >> 1) * 8 >= count) {
-#pragma unroll
-                        for (int w = 0; w < kWords; ++w) word[i][w] = 0u;
-                    }
-                }
-            }
-#pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t a[4];
-                    to_half<C::kInt8>(__byte_perm(word[0][w], word[1][w], h == 0 ? 0x5140 : 0x7362), a[0], a[1]);
-                    to_half<C::kInt8>(__byte_perm(word[2][w], word[3][w], h == 0 ? 0x5140 : 0x7362), a[2], a[3]);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma(o[2 * w + h][n], a, weight[n][0], weight[n][1]);
-                }
-            }
-        }
+        };
+        if (NT == 1 && fold) take_units(std::true_type{});
+        else take_units(std::false_type{});
 
         // ---- the warps' results are joined, while the next piece's units are on their way ----
         const int done_first = q.first, done_queries = q.queries, done_head = head, done_query0 = query0;
-        const bool done_whole = whole;
+        const bool done_whole = whole, done_fold = fold;
         if (more_spans > 0 && tid == 0) p.cuts[blockIdx.x] = {more_spans + 1, static_cast<int>(slot & 1), q.first, q.queries - query0, query0, head};
         const int64_t done_slot = slot;
         more = next_piece();
@@ -678,7 +709,12 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    const float4 part = *reinterpret_cast<const float4*>(smem + (w * kStages + __float_as_int(stat[w].w)) * C::kStage + (column * D + channel) * 4);
+                    const uint8_t* sums = smem + (w * kStages + __float_as_int(stat[w].w)) * C::kStage + (column * D + channel) * 4;
+                    float4 part = *reinterpret_cast<const float4*>(sums);
+                    if (done_fold) {
+                        const float4 lower = *reinterpret_cast<const float4*>(sums + 4 * D * 4);
+                        part = make_float4(part.x + lower.x, part.y + lower.y, part.z + lower.z, part.w + lower.w);
+                    }
                     const float share = exp2_fast(stat[w].z - M_all);
                     l_all += stat[w].y * exp2_fast(stat[w].x - m_all);
                     sum.x += part.x * share;
