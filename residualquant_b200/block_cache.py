@@ -182,15 +182,15 @@ class BlockCache:
         front = (*self._view, *batch, query_address, output_address, query_stride, output_stride, rows, heads, _ACTIVATIONS[query.dtype],
                  bool(accumulate), scale, lse.data_ptr() if lse is not None else 0, min(max_seq_len or 0, 0x7FFFFFFF))
         sizes = (rows, heads, batch[3], batch[5], bool(accumulate), max_seq_len)
-        nbytes = self._workspaces.get(sizes)
-        if nbytes is None:
-            nbytes = self._lib.rq_block_attention_workspace_bytes(_ATTENTION.pack(*front, 0, 0, 0, 0))
-            if len(self._workspaces) >= 4096:
-                self._workspaces.clear()
-            self._workspaces[sizes] = nbytes
+        known = self._workspaces.get(sizes)
+        nbytes = known if known is not None else self._lib.rq_block_attention_workspace_bytes(_ATTENTION.pack(*front, 0, 0, 0, 0))
         workspace = self.codes.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         self._call(self._lib.rq_block_attention,
                    _ATTENTION.pack(*front, workspace.data_ptr() if nbytes else 0, nbytes, self._stream(), 0))
+        if known is None:  # only now: of arguments that the call refuses the size is 0
+            if len(self._workspaces) >= 4096:
+                self._workspaces.clear()
+            self._workspaces[sizes] = nbytes
 
     def attention_status(self) -> None:
         """Synchronize and raise if a bounded wait inside an attention kernel of any block cache ever gave up on this device."""

@@ -123,3 +123,60 @@ def test_the_cache_lives_on_the_gpu(built_library):
         BlockCache(codes, torch.ones(2, 4, 2))
     with pytest.raises(RuntimeError):
         BlockCache.allocate(4, 2, 64, device="cpu")
+
+
+class HostCache(BlockCache):
+    """A cache over CPU tensors whose attention calls end at the library's checks: `asked` are the workspace sizes that accepted calls
+    came with, `devices` the devices that were current while the library was asked for sizes or called."""
+
+    def __init__(self, monkeypatch, width):
+        lib = _lib.load()
+        self.codes, self.scales, self.weights = torch.zeros(2, 4, 2, 16, 64, dtype=torch.int8), torch.ones(2, 4, 2), None
+        self.num_blocks, self.kv_heads, self.block_size, self.head_dim = 4, 2, 16, 64
+        self.device, self._workspaces = self.codes.device, {}
+        self._view = (self.codes.data_ptr(), self.scales.data_ptr(), 0, 4, 2, 64, 16, 1)
+        self._lib, self.asked, self.devices = self, [], []
+        self.batch = torch.tensor([0, 1]).int(), torch.tensor([5]).int(), torch.zeros(1, width, dtype=torch.int32)
+        self.current = [7]                                     # not this cache's
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: self.current[-1])
+
+        class Device:
+            def __init__(device, index):
+                device.index = index
+
+            def __enter__(device):
+                self.current.append(device.index)
+
+            def __exit__(device, *_):
+                self.current.pop()
+
+        monkeypatch.setattr(torch.cuda, "device", Device)
+        self.need = lib.rq_block_attention_workspace_bytes
+
+    def _stream(self):
+        return 0
+
+    def rq_block_attention_workspace_bytes(self, args):
+        self.devices.append(self.current[-1])
+        return self.need(args)
+
+    def rq_block_attention(self, args):
+        self.devices.append(self.current[-1])
+        given = _lib.RqBlockAttentionArgs.from_buffer_copy(args)
+        need = self.need(args)
+        if need == 0:
+            return -1                                          # a table this wide needs one: the arguments are not valid
+        self.asked.append((given.workspace_bytes, need))
+        return 0
+
+
+@pytest.mark.parametrize("refused", [dict(softmax_scale=1e-60), dict(expand=True)])
+def test_a_refused_call_leaves_later_ones_alone(built_library, monkeypatch, refused):
+    cache = HostCache(monkeypatch, 100)
+    query = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    bad = query[:1].expand(2, 4, 64) if refused.get("expand") else query
+    with pytest.raises(RuntimeError):
+        cache.attention(bad, query, *cache.batch, softmax_scale=refused.get("softmax_scale"))
+    for _ in range(2):
+        cache.attention(query, query, *cache.batch)
+    assert len(cache.asked) == 2 and all(given == need > 0 for given, need in cache.asked)
