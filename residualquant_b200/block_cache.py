@@ -116,12 +116,14 @@ class BlockCache:
     def _stream(self) -> int:
         return torch._C._cuda_getCurrentRawStream(self.device.index)
 
-    def _call(self, function, args: bytes) -> None:
+    def _on_device(self, function, args: bytes) -> int:
         if torch.cuda.current_device() == self.device.index:
-            status = function(args)
-        else:
-            with torch.cuda.device(self.device.index):
-                status = function(args)
+            return function(args)
+        with torch.cuda.device(self.device.index):
+            return function(args)
+
+    def _call(self, function, args: bytes) -> None:
+        status = self._on_device(function, args)
         if status != _lib.RQ_OK:
             _lib.check(status)
 
@@ -183,7 +185,9 @@ class BlockCache:
                  bool(accumulate), scale, lse.data_ptr() if lse is not None else 0, min(max_seq_len or 0, 0x7FFFFFFF))
         sizes = (rows, heads, batch[3], batch[5], bool(accumulate), max_seq_len)
         known = self._workspaces.get(sizes)
-        nbytes = known if known is not None else self._lib.rq_block_attention_workspace_bytes(_ATTENTION.pack(*front, 0, 0, 0, 0))
+        nbytes = known
+        if known is None:  # (it depends on the device's size too)
+            nbytes = self._on_device(self._lib.rq_block_attention_workspace_bytes, _ATTENTION.pack(*front, 0, 0, 0, 0))
         workspace = self.codes.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         self._call(self._lib.rq_block_attention,
                    _ATTENTION.pack(*front, workspace.data_ptr() if nbytes else 0, nbytes, self._stream(), 0))

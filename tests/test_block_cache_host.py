@@ -180,3 +180,10 @@ def test_a_refused_call_leaves_later_ones_alone(built_library, monkeypatch, refu
     for _ in range(2):
         cache.attention(query, query, *cache.batch)
     assert len(cache.asked) == 2 and all(given == need > 0 for given, need in cache.asked)
+
+
+def test_the_workspace_is_sized_on_the_device_of_the_cache(built_library, monkeypatch):
+    cache = HostCache(monkeypatch, 100)
+    query = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    cache.attention(query, query, *cache.batch)
+    assert cache.devices == [cache.device.index] * 2 and cache.current == [7]
