@@ -304,8 +304,9 @@ int32_t rq_peer_barrier_status(const void* state, void* stream);
  *            positive finite value
  *   weights  fp32 [num_blocks][kv_heads][page_tokens]: accumulated attention weight of every cached token, or NULL
  * Token t of request r lives in block block_table[r][t / page_tokens] at slot t % page_tokens, for every KV head.
- * No two requests of one call may share a block that the call writes.  A block id outside 0..num_blocks-1 is never
- * dereferenced: tokens in such a block are invisible to attention, not written by append, and lost by evict. */
+ * A block table is at most 2^30 tokens wide.  No two requests of one call may share a block that the call writes.  A block
+ * id outside 0..num_blocks-1 is never dereferenced: tokens in such a block are invisible to attention, not written by
+ * append, and lost by evict. */
 typedef enum RqBlockElement { RQ_BLOCK_E4M3 = 0, RQ_BLOCK_INT8 = 1 } RqBlockElement;
 typedef enum RqActivation { RQ_ACTIVATION_BF16 = 0, RQ_ACTIVATION_FP16 = 1 } RqActivation;
 

@@ -125,6 +125,23 @@ def test_the_cache_lives_on_the_gpu(built_library):
         BlockCache.allocate(4, 2, 64, device="cpu")
 
 
+@pytest.mark.parametrize("page", [16, 32])
+def test_a_table_of_more_than_2_to_the_30_tokens_is_refused(built_library, page):
+    lib = _lib.load()
+    most = (1 << 30) // page
+
+    def table(pages):
+        return dict(page_tokens=page, block_table_stride=pages, max_blocks_per_request=pages)
+
+    assert 0 < lib.rq_block_attention_workspace_bytes(ctypes.byref(attention_args(**table(most)))) < 1 << 30
+    assert lib.rq_block_append(ctypes.byref(append_args(**table(most)))) == 0                       # no rows
+    for pages in (most + 1, 0x7FFFFFFF // page, 0x7FFFFFFF):
+        assert lib.rq_block_attention_workspace_bytes(ctypes.byref(attention_args(**table(pages)))) == 0
+        assert lib.rq_block_attention(ctypes.byref(attention_args(num_rows=0, **table(pages)))) == -1
+        assert lib.rq_block_append(ctypes.byref(append_args(**table(pages)))) == -1
+        assert lib.rq_block_evict(ctypes.byref(evict_args(budget=4, **table(pages)))) == -1
+
+
 class HostCache(BlockCache):
     """A cache over CPU tensors whose attention calls end at the library's checks: `asked` are the workspace sizes that accepted calls
     came with, `devices` the devices that were current while the library was asked for sizes or called."""
