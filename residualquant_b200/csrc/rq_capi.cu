@@ -812,7 +812,9 @@ int32_t rq_block_evict(const RqBlockEvictArgs* a) {
         return fail(RQ_ERR_INVALID_ARGUMENT, "a budget of %d tokens cannot hold the first %d and the last %d", a->budget, a->sinks, a->recent);
     if (a->kept == nullptr || !aligned(a->kept, 4) || !aligned(a->new_lens, 4))
         return fail(RQ_ERR_INVALID_ARGUMENT, "int32 [requests, heads, budget] for the kept positions required");
-    if (a->new_lens == a->batch.seq_lens) return fail(RQ_ERR_INVALID_ARGUMENT, "new_lens must not be seq_lens itself");
+    const int64_t apart = reinterpret_cast<intptr_t>(a->new_lens) - reinterpret_cast<intptr_t>(a->batch.seq_lens);
+    if (a->new_lens != nullptr && apart > -4LL * a->batch.num_requests && apart < 4LL * a->batch.num_requests)
+        return fail(RQ_ERR_INVALID_ARGUMENT, "new_lens must not share memory with seq_lens");
     const int64_t pairs = static_cast<int64_t>(a->batch.num_requests) * a->cache.kv_heads;
     if (pairs > 0x7fffffffLL / 64) return fail(RQ_ERR_INVALID_ARGUMENT, "too many requests in one call");
     p.budget = a->budget;

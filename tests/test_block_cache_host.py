@@ -142,6 +142,14 @@ def test_a_table_of_more_than_2_to_the_30_tokens_is_refused(built_library, page)
         assert lib.rq_block_evict(ctypes.byref(evict_args(budget=4, **table(pages)))) == -1
 
 
+@pytest.mark.parametrize("offset,shared", [(-4, True), (0, True), (4, True), (4 * (1 << 30) - 4, True), (4 * (1 << 30), False)])
+def test_new_lengths_that_share_memory_with_the_lengths_are_refused(built_library, offset, shared):
+    lib = _lib.load()
+    # 2^30 requests are too many in any case, so that nothing is launched; what is said first is the overlap
+    assert lib.rq_block_evict(ctypes.byref(evict_args(budget=4, new_lens=ADDRESS + offset, num_requests=1 << 30))) == -1
+    assert (b"seq_lens" in lib.rq_last_error()) == shared
+
+
 class HostCache(BlockCache):
     """A cache over CPU tensors whose attention calls end at the library's checks: `asked` are the workspace sizes that accepted calls
     came with, `devices` the devices that were current while the library was asked for sizes or called."""
