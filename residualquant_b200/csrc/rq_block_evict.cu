@@ -59,7 +59,7 @@ __device__ __forceinline__ uint32_t move_codes(uint32_t word, __half2 ratio) {
 }
 
 struct EvictShared {
-    uint32_t histogram[kBins];
+    alignas(16) uint32_t histogram[kBins];          // read in pieces of 16 bytes
     uint32_t greater[kMaxWarps], equal[kMaxWarps];  // a warp's candidates above / at the threshold
     uint32_t digit, above;                          // digit found by a pass, candidates above it
     uint32_t slice;                                 // candidates of all CTAs in this CTA's slice of the bins
