@@ -9,6 +9,8 @@
 // request's first row, or one whose position starts a block); the tokens stay in registers between the maximum and the
 // encoding, so every row is read once.  Finding the request, position and page costs three dependent loads, so a warp goes on
 // to other heads and planes of the block where there are warps enough.  Memory bound: 2 bytes read and 1 written per element.
+#include <type_traits>
+
 #include "rq_block_common.cuh"
 
 namespace rq {
@@ -16,7 +18,7 @@ namespace {
 
 constexpr int kAppendWarps = 8;
 
-// Eight activations -> eight codes, for finite values that the scale brings into range.
+// Eight activations -> eight codes, for finite values that the scale, a power of two, brings into range.
 template <bool INT8>
 __device__ __forceinline__ uint2 encode8_finite(const uint4& x, float inverse, bool fp16) {
     const uint32_t words[4] = {x.x, x.y, x.z, x.w};
@@ -35,18 +37,43 @@ __device__ __forceinline__ uint2 encode8_finite(const uint4& x, float inverse, b
     return make_uint2(__byte_perm(pairs[0], pairs[1], 0x5410), __byte_perm(pairs[2], pairs[3], 0x5410));
 }
 
-// The same with infinities and NaN among them.
+// The same with infinities and NaN among them, or a scale of any value that the block had before.
 template <bool INT8>
-__device__ __noinline__ uint2 encode8(uint4 x, float inverse, bool fp16) {
-    const float2 a = activation2(x.x, fp16), b = activation2(x.y, fp16), c = activation2(x.z, fp16), d = activation2(x.w, fp16);
-    return make_uint2(encode2<INT8>(a.x * inverse, a.y * inverse) | (encode2<INT8>(b.x * inverse, b.y * inverse) << 16),
-                      encode2<INT8>(c.x * inverse, c.y * inverse) | (encode2<INT8>(d.x * inverse, d.y * inverse) << 16));
+__device__ __noinline__ uint2 encode8(uint4 x, float scale, float inverse, bool fp16) {
+    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+    uint32_t pairs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = activation2(words[i], fp16);
+        pairs[i] = encode2<INT8>(sided_quotient(f.x, scale, inverse), sided_quotient(f.y, scale, inverse));
+    }
+    return make_uint2(pairs[0] | (pairs[1] << 16), pairs[2] | (pairs[3] << 16));
 }
 
 // Largest of two pairs' 16-bit magnitudes, pair by pair.
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b & 0x7fff7fffu); }
+
+// The codes of a block's first `old` tokens under a scale that grew.
 template <int D, int P, bool INT8>
-__global__ void __launch_bounds__(kAppendWarps * 32) block_append_kernel(const BlockAppendParams p) {
+__device__ __noinline__ void round_again(uint8_t* page, int old, float ratio) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kPieces = P * D / 256;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int piece = i * 32 + lane;
+        if (piece / (D / 8) < old) {
+            uint2* at = reinterpret_cast<uint2*>(page + piece * 8);
+            const uint2 c = *at;
+            *at = make_uint2(rescale4<INT8>(c.x, ratio), rescale4<INT8>(c.y, ratio));
+        }
+    }
+}
+
+// CTAs on a multiprocessor: the registers that a block's pieces take leave room for four, three or two.
+constexpr int append_resident(int block_bytes) { return block_bytes <= 16 * 96 ? 4 : block_bytes <= 16 * 128 ? 3 : 2; }
+
+template <int D, int P, bool INT8>
+__global__ void __launch_bounds__(kAppendWarps * 32, append_resident(P * D)) block_append_kernel(const BlockAppendParams p) {
     constexpr int kRow = D / 8;             // pieces of eight channels in a row
     constexpr int kPieces = P * kRow / 32;  // pieces of a block that a lane holds
     const BlockView& v = p.v;
@@ -116,26 +143,23 @@ __global__ void __launch_bounds__(kAppendWarps * 32) block_append_kernel(const B
             float scale = fmaxf(amax != 0u ? block_scale<INT8>(amax) : 0.f, before);
             if (scale == 0.f) scale = 1.f;
             if (old != 0 && scale > before) {
-                const float ratio = before / scale;
+                round_again<D, P, INT8>(page, old, before / scale);
+            }
+            // every scale written here is a power of two, but the block may have come with another
+            const bool plain = finite && power_of_two(scale);
+            const float inverse = 1.f / scale;
+            auto write_codes = [&](auto finite_power) {
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
-                    const int piece = i * 32 + lane;
-                    if (piece / kRow < old) {
-                        uint2* at = reinterpret_cast<uint2*>(page + piece * 8);
-                        const uint2 c = *at;
-                        const float2 a = decode2<INT8>(c.x), b = decode2<INT8>(c.x >> 16), d = decode2<INT8>(c.y), e = decode2<INT8>(c.y >> 16);
-                        *at = make_uint2(encode2<INT8>(a.x * ratio, a.y * ratio) | (encode2<INT8>(b.x * ratio, b.y * ratio) << 16),
-                                         encode2<INT8>(d.x * ratio, d.y * ratio) | (encode2<INT8>(e.x * ratio, e.y * ratio) << 16));
+                    const int piece = i * 32 + lane, token = piece / kRow - old;
+                    if (token >= 0 && token < count) {
+                        if constexpr (decltype(finite_power)::value) *reinterpret_cast<uint2*>(page + piece * 8) = encode8_finite<INT8>(x[i], inverse, p.fp16);
+                        else *reinterpret_cast<uint2*>(page + piece * 8) = encode8<INT8>(x[i], scale, inverse, p.fp16);
                     }
                 }
-            }
-            const float inverse = 1.f / scale;  // exact: the scales written here are powers of two
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int piece = i * 32 + lane, token = piece / kRow - old;
-                if (token >= 0 && token < count)
-                    *reinterpret_cast<uint2*>(page + piece * 8) = finite ? encode8_finite<INT8>(x[i], inverse, p.fp16) : encode8<INT8>(x[i], inverse, p.fp16);
-            }
+            };
+            if (plain) write_codes(std::true_type{});
+            else write_codes(std::false_type{});
             __syncwarp();  // every lane has read the scale
             if (lane == 0) *scale_at = scale;
             if (plane == 0 && v.weights != nullptr && lane < count) v.weights[(id * v.kv_heads + head) * P + old + lane] = 0.f;

@@ -19,6 +19,21 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
     return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
+__device__ __forceinline__ bool power_of_two(float x) { return (__float_as_uint(x) & 0x7fffffu) == 0u; }  // of a normal x
+
+// A product, and a quotient given the divisor's approximate inverse, in a form that rounds to the few bits of a code as the exact
+// values would, ties included: a number next to it on the same side of every shorter number, or itself where that is exact.
+__device__ __forceinline__ float sided_product(float a, float b) {
+    const float p = __fmul_rz(a, b);  // and the last bit set where anything was left over
+    return fabsf(fmaf(a, b, -p)) > 0.f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+}
+__device__ __forceinline__ float sided_quotient(float a, float b, float inverse) {
+    const float q = a * inverse, t = __uint_as_float((__float_as_uint(q) + 0x80u) & 0xffffff00u);  // 16 bits of it
+    const float left = fmaf(-t, b, a);                                                            // its sign is exact
+    if (!(fabsf(left) > 0.f)) return left == 0.f ? t : q;                                         // infinities and NaN: q
+    return __uint_as_float(__float_as_uint(t) + ((left > 0.f) == (__float_as_int(t) >= 0) ? 1u : ~0u));
+}
+
 // Two cached bytes -> two floats (exact).
 template <bool INT8>
 __device__ __forceinline__ float2 decode2(uint32_t pair) {
@@ -39,6 +54,14 @@ __device__ __forceinline__ uint32_t encode2(float a, float b) {
         const float2 v = make_float2(a == a ? a : 0.f, b == b ? b : 0.f);
         return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
     }
+}
+
+// Four codes times any ratio, rounded to codes again once.
+template <bool INT8>
+__device__ __forceinline__ uint32_t rescale4(uint32_t word, float ratio) {
+    const float2 a = decode2<INT8>(word), b = decode2<INT8>(word >> 16);
+    return encode2<INT8>(sided_product(a.x, ratio), sided_product(a.y, ratio)) |
+           (encode2<INT8>(sided_product(b.x, ratio), sided_product(b.y, ratio)) << 16);
 }
 
 // Four cached bytes -> two fp16 pairs (bytes 0, 1 and bytes 2, 3), exact.  int8: a byte with its sign bit flipped is
