@@ -58,6 +58,12 @@ __device__ __forceinline__ uint32_t move_codes(uint32_t word, __half2 ratio) {
     }
 }
 
+// The same for any ratio (not inlined: 32 sequences of 4097 to 9001 tokens take 142 us, inlined 145).
+template <bool INT8>
+__device__ __noinline__ uint32_t move_codes_any(uint32_t word, float ratio) {
+    return rescale4<INT8>(word, ratio);
+}
+
 struct EvictShared {
     alignas(16) uint32_t histogram[kBins];          // read in pieces of 16 bytes
     uint32_t greater[kMaxWarps], equal[kMaxWarps];  // a warp's candidates above / at the threshold
@@ -327,7 +333,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
                 largest = __hmax2(largest, __hmax2(__habs2(*reinterpret_cast<__half2*>(&low)), __habs2(*reinterpret_cast<__half2*>(&high))));
             }
             const float2 both = __half22float2(largest);
-            const uint32_t bits = __float_as_uint(fmaxf(both.x, both.y) * __shfl_sync(kFullMask, now.scale, (i * 32 + lane) / kRow));
+            const uint32_t bits = __float_as_uint(__fmul_ru(fmaxf(both.x, both.y), __shfl_sync(kFullMask, now.scale, (i * 32 + lane) / kRow)));
             if (bits < 0x7f800000u) amax = max(amax, bits);
         }
         amax = __reduce_max_sync(kFullMask, amax);
@@ -350,10 +356,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, P == 16 ? 2 : 1) block_evict_k
                 for (int j = 0; j < 4; ++j) words[j] = move_codes<INT8>(words[j], half_ratio);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 a = decode2<INT8>(words[j]), b = decode2<INT8>(words[j] >> 16);
-                    words[j] = encode2<INT8>(a.x * ratio, a.y * ratio) | (encode2<INT8>(b.x * ratio, b.y * ratio) << 16);
-                }
+                for (int j = 0; j < 4; ++j) words[j] = move_codes_any<INT8>(words[j], ratio);
             }
             if (write && piece / kRow < now.count)
                 *reinterpret_cast<uint4*>(v.codes + plane_page * P * D + piece * 16) = make_uint4(words[0], words[1], words[2], words[3]);

@@ -1,4 +1,4 @@
-"""Blocks that come with scales that are no powers of two: append rounds to the codes of the definition, to the bit, where
+"""Blocks that come with scales that are no powers of two: append and evict round to the codes of the definition, to the bit, where
 fp32 products and reciprocals end on the wrong side of a tie."""
 
 import numpy as np
@@ -83,4 +83,25 @@ def test_append_rounds_earlier_tokens_again_from_a_scale_of_any_value(dtype, dim
     cache.append(key, -key, *(ints(a) for a in args))
     oracle.append(key, -key, *args)
     assert torch.all(cache.scales == 1.0)
+    same_cache(cache, oracle)
+
+
+@pytest.mark.parametrize("border", [False, True])
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("dim,page", [(128, 16), (96, 32), (64, 32)])
+def test_evict_from_blocks_with_scales_of_any_value(dtype, dim, page, border):
+    """`border`: the largest value is above the range by less than fp32 shows, so the next power of two is needed."""
+    found = near_ties(dtype, border)[:100]
+    assert len(found) > 3
+    cache = BlockCache.allocate(2 * len(found), 1, dim, page, dtype, weights=True)
+    for i, (code, ratio) in enumerate(found):
+        largest = code if border else CODES[dtype][-1]
+        cache.codes[:, 2 * i:2 * i + 2] = raw(np.resize([code, -code, largest, CODES[dtype][0]], (page, dim)), dtype)
+        cache.scales[:, 2 * i:2 * i + 2] = ratio
+    cache.weights.copy_(torch.rand(cache.weights.shape, generator=torch.Generator().manual_seed(1)))
+    oracle = oracle_of(cache)
+    lengths, table = [page + 5] * len(found), [[2 * i, 2 * i + 1] for i in range(len(found))]
+    kept, _ = cache.evict(ints(lengths), ints(table), page - 3, recent=2)
+    want, _ = oracle.evict(lengths, table, page - 3, 0, 2)
+    assert torch.equal(kept.cpu(), want)
     same_cache(cache, oracle)
