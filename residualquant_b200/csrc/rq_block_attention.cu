@@ -281,6 +281,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the barriers are there for the copies
     __syncwarp();
     uint32_t phases = 0u;  // bit s: parity of the copy into stage s that is waited for next
+    bool failed = false;   // a copy has not arrived in time
 
     // The span's pieces, one after the other; all of this but `units` is the same in every thread of the block.
     int64_t at = begin;
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
         }
         const int id = __shfl_sync(kFullMask, ids, unit & 31);
         const int token0 = token_begin + (warp + unit * kWarps) * kUnit;
-        if (lane == 0) {
+        if (lane == 0 && !failed) {
             const uint32_t barrier = barriers + to * 8;
             barrier_expect(barrier, id >= 0 ? C::kStage : 0);
             if (id >= 0) {
@@ -390,7 +391,6 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) produce(i, stage + i < kStages ? stage + i : stage + i - kStages);
     };
-    bool failed = false;
     bool more = next_piece();
     if (more) {
         set_off();
@@ -738,9 +738,11 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
             __syncthreads();  // the sums have been read: their stages are free
         }
     }
-    if (failed) {  // a copy did not arrive in time (no case is known): the call's results are not to be used
+    // A copy did not arrive in time (no case is known): the call's results are not to be used.  None was set off after that, and
+    // the limit passes once more, for those that were on their way, before the shared memory is given up.
+    if (failed) {
         atomicExch(&g_block_attention_status, RQ_ERR_DEVICE_TIMEOUT);
-        for (uint32_t polls = 0; polls < kWaitLimit && !barrier_done(barriers + stage * 8, phases >> stage & 1u); ++polls) {}
+        for (uint32_t polls = 0; polls < kWaitLimit; ++polls) static_cast<void>(barrier_done(barriers + stage * 8, phases >> stage & 1u));
     }
 }
 
