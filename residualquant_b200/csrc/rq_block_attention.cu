@@ -113,6 +113,12 @@ __device__ __forceinline__ bool barrier_done(uint32_t barrier, uint32_t parity) 
                  : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
     return done != 0;
 }
+// A copy did not arrive in time (no case is known): the call's results are not to be used.  No copy was set off after that, and
+// the limit passes once more, for those that were on their way, before the shared memory is given up.
+__device__ __noinline__ void give_up(uint32_t barrier) {
+    atomicExch(&g_block_attention_status, RQ_ERR_DEVICE_TIMEOUT);
+    for (uint32_t polls = 0; polls < kWaitLimit; ++polls) static_cast<void>(barrier_done(barrier, 0u));
+}
 // kUnit tokens of a head from one page, rows row .. row + 15 of block `block` of the map.
 __device__ __forceinline__ void copy_unit(uint32_t to, const CUtensorMap* map, int row, int block, uint32_t barrier) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -738,12 +744,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
             __syncthreads();  // the sums have been read: their stages are free
         }
     }
-    // A copy did not arrive in time (no case is known): the call's results are not to be used.  None was set off after that, and
-    // the limit passes once more, for those that were on their way, before the shared memory is given up.
-    if (failed) {
-        atomicExch(&g_block_attention_status, RQ_ERR_DEVICE_TIMEOUT);
-        for (uint32_t polls = 0; polls < kWaitLimit; ++polls) static_cast<void>(barrier_done(barriers + stage * 8, phases >> stage & 1u));
-    }
+    if (failed) give_up(barriers);
 }
 
 // Joins the pieces of the items that more than one span took part in.  At most one such item begins in a span; the CTAs of
