@@ -300,8 +300,8 @@ int32_t rq_peer_barrier_status(const void* state, void* stream);
  * A paged cache for KV owners that are not residual-coded (no counterpart in the reference, which keeps them in bf16):
  * one byte per channel and one fp32 scale per (plane, block, KV head).  A cached value is code * scale.
  *   codes    e4m3 or int8 [2][num_blocks][kv_heads][page_tokens][head_dim], plane 0 = K, plane 1 = V
- *   scales   fp32 [2][num_blocks][kv_heads]; rq_block_append and rq_block_evict write powers of two, attention reads any
- *            positive finite value
+ *   scales   fp32 [2][num_blocks][kv_heads]; rq_block_append and rq_block_evict write powers of two, and take any positive
+ *            finite value that a block comes with, as attention does (append keeps one that is large enough)
  *   weights  fp32 [num_blocks][kv_heads][page_tokens]: accumulated attention weight of every cached token, or NULL
  * Token t of request r lives in block block_table[r][t / page_tokens] at slot t % page_tokens, for every KV head.
  * A block table is at most 2^30 tokens wide.  No two requests of one call may share a block that the call writes.  A block

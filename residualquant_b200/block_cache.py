@@ -14,7 +14,7 @@ no fixed order).
 
 A cached value is code * scale.  `append` and `evict` write scales that are powers of two: the smallest one that brings a block's
 largest finite magnitude into the codes' range (448 for float8_e4m3fn, 127 for int8); infinities saturate and NaN is stored as 0.
-`attention` reads any positive finite scales and finite codes.
+All three read any positive finite scales and finite codes (`append` keeps a block's scale, whatever it is, where it is large enough).
 
 Nothing here but `attention_status` synchronizes, and every other call can be captured in a CUDA graph.  Calls go to the current
 stream of the cache's device; scratch memory is taken from PyTorch's allocator for each call, so calls on different streams share
@@ -206,7 +206,8 @@ class BlockCache:
         """Bring every request of more than `budget` tokens down to `budget`, for each KV head on its own: the first `sinks` tokens,
         the last `recent` ones and those of the others with the largest accumulated weight (ties: the lowest position, NaN
         last) move, in their order, to the first `budget` positions of the request's blocks, with their weights.  Requests of at
-        most `budget` tokens are left alone.  The blocks behind ceil(budget / block size) can be given back.
+        most `budget` tokens are left alone.  This cache no longer needs the blocks behind ceil(budget / block size); owners that share
+        the block table and are not evicted with it do, and keep their own lengths.
 
         Returns `kept` int32 [requests, kv heads, budget], the positions that the tokens now at 0, 1, ... had before (-1 behind
         the last), and `new_lens` int32 [requests], min(seq_len, budget); both can be passed in (not `seq_lens` itself)."""

@@ -5,7 +5,8 @@
 // queries fill an instruction:
 //     S^T [16 tokens x 8 queries]  = K [16 x D] Q^T              (mma m16n8k16, fp16 inputs, fp32 sums)
 //     O^T [16 channels x 8 queries] += V^T [16 x 16 tokens] P^T
-// Codes become fp16 exactly, and queries too: each is brought into fp16's range by a power of two.  Which channel an
+// Codes become fp16 exactly; a query is brought into fp16's range by a power of two, which costs channels below 2^-28 of its
+// largest some of their bits.  Which channel an
 // instruction's k index means is free as long as both sides agree, so every thread takes whole 8- or 16-byte pieces of a
 // row; V's token pairs are interleaved with byte permutes.  The block scales multiply the scores (K) and go into the
 // exponent of the softmax weights (V).
@@ -51,7 +52,8 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;              // tokens of one mma step
 constexpr int kChunk = kWarps * kUnit; // tokens that spans are counted in
 constexpr int kItemCost = 3;           // chunks' worth of time that a CTA spends on beginning and ending an item
-constexpr int resident(int query_tiles) { return query_tiles == 1 ? 4 : 3; }  // CTAs on a multiprocessor: registers for four or three
+// CTAs on a multiprocessor: registers for four or three (128 or 168 a thread; 128 channels spill 32 to 88 bytes at that).
+constexpr int resident(int query_tiles) { return query_tiles == 1 ? 4 : 3; }
 constexpr int kJoinWarps = 8;
 constexpr uint32_t kWaitLimit = 1u << 22;  // polls of a copy's barrier before the kernel gives up
 constexpr float kNever = -1e30f;       // reference of a query that has seen no token
@@ -436,7 +438,8 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
             uint32_t amax = __float_as_uint(activation2(bits, p.fp16).x);
             amax = max(amax, __shfl_xor_sync(kFullMask, amax, 1));
             amax = max(amax, __shfl_xor_sync(kFullMask, amax, 2));
-            // the largest magnitude goes to [2^14, 2^15): exact for everything down to 2^-39 of it
+            // The largest magnitude goes to [2^14, 2^15).  bf16 channels down to 2^-31 of it and fp16 ones down to 2^-28 stay
+            // exact; smaller ones are off by at most 2^-25, half a step of fp16 there, or 2^-39 of the largest.
             const int e = amax == 0u ? 0 : max(static_cast<int>(amax >> 23) - 127 - 14, -120);
             const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
@@ -750,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, resident(C::NT)) block_attention_ker
 // Joins the pieces of the items that more than one span took part in.  At most one such item begins in a span; the CTAs of
 // row `part` of the grid take every gridDim.y-th of its queries, all of their warps on as few at a time as leave none out.
 // kBatch pieces are on their way to a warp at once: many where one item is cut into hundreds, few registers (and all CTAs
-// resident) where many are cut in two.
+// resident: 40 registers for six, 48 bytes spilled) where many are cut in two.
 template <typename C, int kBatch>
 __global__ void __launch_bounds__(kJoinWarps * 32, kBatch > 2 ? 2 : 6) block_join_kernel(const BlockAttentionParams p) {
     constexpr int D = C::D, kRows = C::kRows, kLanes = D / 4;

@@ -824,7 +824,9 @@ int32_t rq_block_evict(const RqBlockEvictArgs* a) {
     p.new_lens = a->new_lens;
     // CTAs per (request, KV head): as many (up to eight) as the multiprocessors leave and as have at least 1024 of the tokens
     // each that a request can have.  Sixteen-warp CTAs where there is at most one for each multiprocessor, else eight-warp
-    // ones, of which three or four fit (8 sequences x 30000 tokens x 8 heads: 95 instead of 112 us).
+    // ones, of which three fit with pages of 16 (shared memory) and two or three with pages of 32 (registers).  Eight / sixteen
+    // warps, 128 channels: 64 sequences x 4500 tokens x 16 heads 232 / 246 us with pages of 16, 251 / 279 with pages of 32;
+    // 8 x 30000 x 8 heads 96 / 88 and 85 / 100.
     const int64_t most = static_cast<int64_t>(p.v.max_blocks) * p.v.page_tokens;
     p.cluster = 1;
     while (p.cluster < 8 && pairs * p.cluster <= current_sm_count() && most / (2 * p.cluster) >= 1024) p.cluster *= 2;
