@@ -643,6 +643,8 @@ static int block_view(const RqBlockCache& c, const RqBlockBatch& b, bool rows, r
         return fail(RQ_ERR_INVALID_ARGUMENT, "16-byte aligned 8-bit codes [2, blocks, heads, page tokens, channels], fp32 scales and 16-byte aligned weights required");
     if (b.num_requests < 1 || b.seq_lens == nullptr || (b.block_table == nullptr && b.max_blocks_per_request > 0) || (rows && b.query_start_loc == nullptr))
         return fail(RQ_ERR_INVALID_ARGUMENT, "int32 query starts [requests+1], sequence lengths [requests] and page table required");
+    if (!aligned(b.seq_lens, 4) || !aligned(b.block_table, 4) || (rows && !aligned(b.query_start_loc, 4)))
+        return fail(RQ_ERR_INVALID_ARGUMENT, "4-byte aligned query starts, sequence lengths and page table required");
     if (b.max_blocks_per_request < 0 || b.block_table_stride < b.max_blocks_per_request)
         return fail(RQ_ERR_INVALID_ARGUMENT, "int32 page table with packed rows required");
     // (so that sums of token positions and strides over a table stay in 32 bits)
@@ -719,6 +721,7 @@ static int block_attention_params(const RqBlockAttentionArgs* a, rq::BlockAttent
         return fail(RQ_ERR_INVALID_ARGUMENT, "16-byte aligned 16-bit [tokens, heads, channels] with packed trailing strides required");
     if (!(a->softmax_scale > 0.f && a->softmax_scale < 1e30f)) return fail(RQ_ERR_INVALID_ARGUMENT, "softmax scale must be positive and finite");
     if (a->max_seq_len < 0) return fail(RQ_ERR_INVALID_ARGUMENT, "negative max_seq_len");
+    if (!aligned(a->lse, 4)) return fail(RQ_ERR_INVALID_ARGUMENT, "4-byte aligned lse required");
     if (a->accumulate && a->cache.weights == nullptr) return fail(RQ_ERR_INVALID_ARGUMENT, "accumulating needs a cache with weights");
     if (static_cast<int64_t>(a->batch.num_requests) * a->cache.kv_heads > 0x7fffffffLL / 64)
         return fail(RQ_ERR_INVALID_ARGUMENT, "too many requests in one call");

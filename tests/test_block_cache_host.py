@@ -150,6 +150,27 @@ def test_new_lengths_that_share_memory_with_the_lengths_are_refused(built_librar
     assert (b"seq_lens" in lib.rq_last_error()) == shared
 
 
+@pytest.mark.parametrize("field", ["query_start_loc", "seq_lens", "block_table"])
+def test_metadata_off_their_alignment_are_refused(built_library, field):
+    lib = _lib.load()
+    changes = {field: ADDRESS + 2}
+    assert lib.rq_block_attention(ctypes.byref(attention_args(num_rows=0, **changes))) == -1
+    assert lib.rq_block_append(ctypes.byref(append_args(**changes))) == -1
+    if field != "query_start_loc":
+        # (the second refusal keeps anything from being launched)
+        assert lib.rq_block_evict(ctypes.byref(evict_args(budget=4, kept=ADDRESS + 2, **changes))) == -1
+        assert b"kept" not in lib.rq_last_error()
+
+
+def test_an_lse_off_its_alignment_is_refused(built_library):
+    lib = _lib.load()
+    args = attention_args(num_rows=0)
+    args.lse = ADDRESS + 4
+    assert lib.rq_block_attention(ctypes.byref(args)) == 0
+    args.lse = ADDRESS + 2
+    assert lib.rq_block_attention(ctypes.byref(args)) == -1
+
+
 class HostCache(BlockCache):
     """A cache over CPU tensors whose attention calls end at the library's checks: `asked` are the workspace sizes that accepted calls
     came with, `devices` the devices that were current while the library was asked for sizes or called."""
